@@ -128,7 +128,14 @@ int launch_gather_reduce(const __half* out2, const int32_t* slot_to_row, const f
                 out2, slot_to_row, topk_w, static_cast<float*>(out), N, top_k);
         return launch_status();
     }
-    const dim3 grid((unsigned)((N + 511) / 512), (unsigned)M);    return launch_status();
+    const dim3 grid((unsigned)((N + 511) / 512), (unsigned)M);
+    if (out_half)
+        gather_reduce_kernel<__half><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w,
+                                                               static_cast<__half*>(out), N, top_k);
+    else
+        gather_reduce_kernel<float><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w,
+                                                              static_cast<float*>(out), N, top_k);
+    return launch_status();
 }
 
 }  // namespace w4a8
