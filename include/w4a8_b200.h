@@ -192,6 +192,11 @@ W4A8_API int w4a8_moe_gather_reduce(const void* out2, const int32_t* sorted_toke
                            const float* topk_weights, const int32_t* num_tokens_post_padded,
                            float* out, int64_t M, int64_t N, int64_t P, int64_t top_k,
                            void* workspace, size_t workspace_bytes, w4a8_stream_t stream);
+/* The same with bf16 rows (the block-scaled down product of a bf16 model). */
+W4A8_API int w4a8_moe_gather_reduce_bf16(const void* out2, const int32_t* sorted_token_ids,
+                                const float* topk_weights, const int32_t* num_tokens_post_padded,
+                                float* out, int64_t M, int64_t N, int64_t P, int64_t top_k,
+                                void* workspace, size_t workspace_bytes, w4a8_stream_t stream);
 
 /*
  * silu_and_mul on fp16 rows: x (M, 2*inter) [gate | up] -> out (M, inter),
@@ -307,6 +312,72 @@ W4A8_API int w4a8_moe_decode_packed(const void* x, const int32_t* topk_ids,
                                     int64_t E, const void* p13, const void* p2, int64_t H,
                                     int64_t I, void* out, void* workspace,
                                     size_t workspace_bytes, w4a8_stream_t stream);
+
+/*
+ * Block-scaled FP8: a matrix held as e4m3 bytes with one fp32 scale per block of 128 columns of a
+ * row (activations) or of 128 x 128 (weights); the last block of a side may be short, G =
+ * ceil(K / 128). No counterpart in the reference, whose weights are 4-bit; these serve the layers
+ * that a mixed checkpoint keeps in 8 bits. Type codes: 0 = fp32, 1 = fp16, 2 = bf16.
+ *
+ * w4a8_act_quant_fp8_block: x (M, K) -> q (M, K) e4m3, scales (M, G):
+ *   scales[r, g] = max(amax_{k in block g} |x[r, k]|, 4.48e-6) / 448,  q = e4m3_rn(x / scale),
+ * the rule of w4a8_act_quant_fp8 applied per block. A NaN becomes the e4m3 NaN and does not
+ * enter the amax; a block that holds an infinity gets an infinite scale.
+ */
+W4A8_API int w4a8_act_quant_fp8_block(const void* x, int32_t x_dtype, int64_t M, int64_t K,
+                                      uint8_t* q, float* scales, w4a8_stream_t stream);
+
+/*
+ * RMS norm whose output is quantised as above, in one pass over x (M, H):
+ *   h = round(x + residual) in x's type, stored to residual_out (h = x when residual is NULL;
+ *   residual and residual_out are given together, and residual_out may be residual itself);
+ *   y = h * rsqrt(mean(h^2) + eps) * weight in fp32; q, scales from y;
+ *   normed = round(y) in x's type, when normed is not NULL (the router reads it).
+ * weight (H,) has x's type, or fp32 (weight_dtype 0). q (M, H), scales (M, ceil(H / 128)).
+ */
+W4A8_API int w4a8_rms_norm_quant_fp8(const void* x, const void* residual, const void* weight,
+                                     int32_t x_dtype, int32_t weight_dtype, float eps, int64_t M,
+                                     int64_t H, uint8_t* q, float* scales, void* residual_out,
+                                     void* normed, w4a8_stream_t stream);
+
+/*
+ * Dense block-scaled product: out (M, N) of out_dtype =
+ *   sum_g x_scales[m, g] * w_scales[n / 128, g] * sum_{k in g} x[m, k] * w[n, k],
+ * sums in fp32, rounded once. x (M, K) e4m3, x_scales (M, G); w (N, K) e4m3, w_scales
+ * (ceil(N / 128), G). Any M, N, K; K % 16 == 0 with 16-byte aligned x and w takes the tensor
+ * cores.
+ */
+W4A8_API int w4a8_fp8_block_gemm(const uint8_t* x, const float* x_scales, const uint8_t* w,
+                                 const float* w_scales, void* out, int32_t out_dtype, int64_t M,
+                                 int64_t N, int64_t K, w4a8_stream_t stream);
+
+/*
+ * The same product grouped by expert, on the routing tensors of w4a8_moe_align_block_size: row r
+ * of out (P, N) is activation row sorted_token_ids[r] / top_k times the matrix
+ * expert_ids[r / block_m] of w (E, N, K), w_scales (E, ceil(N / 128), G). sorted_token_ids may be
+ * NULL: x then has P rows, already in sorted order. Padding rows (slot >= T * top_k) and rows of
+ * an expert id outside [0, E) are written as zeros; rows at or past num_tokens_post_padded are
+ * left as they were. block_m is 16, 32, 64 or a multiple of 128.
+ */
+W4A8_API int w4a8_fp8_block_moe_gemm(const uint8_t* x, const float* x_scales, const uint8_t* w,
+                                     const float* w_scales, const int32_t* sorted_token_ids,
+                                     const int32_t* expert_ids,
+                                     const int32_t* num_tokens_post_padded, void* out,
+                                     int32_t out_dtype, int64_t T, int64_t E, int64_t N, int64_t K,
+                                     int64_t P, int64_t top_k, int64_t block_m,
+                                     w4a8_stream_t stream);
+
+/*
+ * Grouped gate_up product fused with SiLU-and-mul and the quantisation that the down product
+ * reads: w (E, 2 * inter, K) = [gate | up]; q (P, inter) e4m3, q_scales (P, inter / 128) of
+ * silu(gate) * up, evaluated in fp32 without a rounding in between. Zero rows (as above) get
+ * q = 0 and the scale of a block of zeros. inter % 128 == 0; the rest as w4a8_fp8_block_moe_gemm.
+ */
+W4A8_API int w4a8_fp8_block_moe_gemm1_silu(
+    const uint8_t* x, const float* x_scales, const uint8_t* w, const float* w_scales,
+    const int32_t* sorted_token_ids, const int32_t* expert_ids,
+    const int32_t* num_tokens_post_padded, uint8_t* q, float* q_scales, int64_t T, int64_t E,
+    int64_t inter, int64_t K, int64_t P, int64_t top_k, int64_t block_m, w4a8_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,8 @@
 //   out[t, n] = sum_{j ascending} w[t*top_k + j] * out2[slot_to_row[t*top_k + j], n]   (fp32)
 // The sum is a plain fp32 multiply then add in slot order, the order the reference oracle uses
 // (w4a8_fp8_wmma/test_moe_experts.py:182-190).
+#include <cuda_bf16.h>
+
 #include <algorithm>
 
 #include "common.cuh"
@@ -13,6 +15,15 @@
 namespace w4a8 {
 
 namespace {
+
+// Row element types: fp16, or bf16 (the rows of a bf16 model's block-scaled down product).
+__device__ __forceinline__ float row_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float row_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename InT>
+__device__ __forceinline__ float2 pair_f32(uint32_t w) {
+    const InT* h = reinterpret_cast<const InT*>(&w);
+    return make_float2(row_f32(h[0]), row_f32(h[1]));
+}
 
 __global__ void build_inverse_map_kernel(const int32_t* __restrict__ sorted_ids,
                                          const int32_t* __restrict__ ntp, int32_t* slot_to_row,
@@ -25,9 +36,9 @@ __global__ void build_inverse_map_kernel(const int32_t* __restrict__ sorted_ids,
 
 // One CTA per (token, 512-channel chunk); each thread reduces 2 adjacent channels. Generic
 // path for N % 8 != 0 or unaligned rows.
-template <typename OutT>
+template <typename InT, typename OutT>
 __global__ void __launch_bounds__(256)
-gather_reduce_kernel(const __half* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
+gather_reduce_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
                      const float* __restrict__ topk_w, OutT* __restrict__ out, int64_t N,
                      int top_k) {
     const int64_t t = blockIdx.y;
@@ -39,14 +50,14 @@ gather_reduce_kernel(const __half* __restrict__ out2, const int32_t* __restrict_
         const int32_t r = slot_to_row[t * top_k + j];
         if (r < 0) continue;
         const float w = topk_w[t * top_k + j];
-        const __half* rowp = out2 + (int64_t)r * N + n;
+        const InT* rowp = out2 + (int64_t)r * N + n;
         if (pair && (N % 2 == 0)) {
-            const __half2 v = *reinterpret_cast<const __half2*>(rowp);
-            a0 = __fadd_rn(a0, __fmul_rn(w, __low2float(v)));
-            a1 = __fadd_rn(a1, __fmul_rn(w, __high2float(v)));
+            const float2 v = pair_f32<InT>(*reinterpret_cast<const uint32_t*>(rowp));
+            a0 = __fadd_rn(a0, __fmul_rn(w, v.x));
+            a1 = __fadd_rn(a1, __fmul_rn(w, v.y));
         } else {
-            a0 = __fadd_rn(a0, __fmul_rn(w, __half2float(rowp[0])));
-            if (pair) a1 = __fadd_rn(a1, __fmul_rn(w, __half2float(rowp[1])));
+            a0 = __fadd_rn(a0, __fmul_rn(w, row_f32(rowp[0])));
+            if (pair) a1 = __fadd_rn(a1, __fmul_rn(w, row_f32(rowp[1])));
         }
     }
     out[t * N + n] = (OutT)a0;
@@ -57,9 +68,9 @@ gather_reduce_kernel(const __half* __restrict__ out2, const int32_t* __restrict_
 // the top_k row indices and weights of the token are staged once per CTA, then every slot's
 // 16-byte row chunk is requested before the in-order accumulation.
 constexpr int kMaxTopK = 16;
-template <typename OutT>
+template <typename InT, typename OutT>
 __global__ void __launch_bounds__(256)
-gather_reduce_vec_kernel(const __half* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
+gather_reduce_vec_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
                          const float* __restrict__ topk_w, OutT* __restrict__ out, int64_t N,
                          int top_k) {
     __shared__ int32_t rows[kMaxTopK];
@@ -87,7 +98,7 @@ gather_reduce_vec_kernel(const __half* __restrict__ out2, const int32_t* __restr
             const uint32_t h[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[c]));
+                const float2 f = pair_f32<InT>(h[c]);
                 acc[2 * c] = __fadd_rn(acc[2 * c], __fmul_rn(w, f.x));
                 acc[2 * c + 1] = __fadd_rn(acc[2 * c + 1], __fmul_rn(w, f.y));
             }
@@ -111,31 +122,31 @@ gather_reduce_vec_kernel(const __half* __restrict__ out2, const int32_t* __restr
 
 }  // namespace
 
-int launch_gather_reduce(const __half* out2, const int32_t* slot_to_row, const float* topk_w,
-                         void* out, bool out_half, int64_t M, int64_t N, int top_k,
-                         cudaStream_t stream) {
+template <typename InT, typename OutT>
+static int launch_reduce(const InT* out2, const int32_t* slot_to_row, const float* topk_w,
+                         OutT* out, int64_t M, int64_t N, int top_k, cudaStream_t stream) {
     if (M <= 0) return W4A8_OK;
     const bool vec = N % 8 == 0 && top_k <= kMaxTopK &&
                      (reinterpret_cast<uintptr_t>(out2) & 15) == 0 &&
                      (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     if (vec) {
         const dim3 grid((unsigned)((N / 8 + 255) / 256), (unsigned)M);
-        if (out_half)
-            gather_reduce_vec_kernel<__half><<<grid, 256, 0, stream>>>(
-                out2, slot_to_row, topk_w, static_cast<__half*>(out), N, top_k);
-        else
-            gather_reduce_vec_kernel<float><<<grid, 256, 0, stream>>>(
-                out2, slot_to_row, topk_w, static_cast<float*>(out), N, top_k);
-        return launch_status();
+        gather_reduce_vec_kernel<InT, OutT><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w,
+                                                                      out, N, top_k);
+    } else {
+        const dim3 grid((unsigned)((N + 511) / 512), (unsigned)M);
+        gather_reduce_kernel<InT, OutT><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w, out,
+                                                                  N, top_k);
     }
-    const dim3 grid((unsigned)((N + 511) / 512), (unsigned)M);
-    if (out_half)
-        gather_reduce_kernel<__half><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w,
-                                                               static_cast<__half*>(out), N, top_k);
-    else
-        gather_reduce_kernel<float><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w,
-                                                              static_cast<float*>(out), N, top_k);
     return launch_status();
+}
+
+int launch_gather_reduce(const __half* out2, const int32_t* slot_to_row, const float* topk_w,
+                         void* out, bool out_half, int64_t M, int64_t N, int top_k,
+                         cudaStream_t stream) {
+    if (out_half)
+        return launch_reduce(out2, slot_to_row, topk_w, static_cast<__half*>(out), M, N, top_k, stream);
+    return launch_reduce(out2, slot_to_row, topk_w, static_cast<float*>(out), M, N, top_k, stream);
 }
 
 }  // namespace w4a8
@@ -144,13 +155,14 @@ extern "C" size_t w4a8_moe_gather_reduce_workspace_size(int64_t M, int64_t top_k
     return w4a8::align_up((size_t)(M * top_k) * sizeof(int32_t), 256);
 }
 
-extern "C" int w4a8_moe_gather_reduce(const void* out2, const int32_t* sorted_token_ids,
-                                      const float* topk_weights,
-                                      const int32_t* num_tokens_post_padded, float* out,
-                                      int64_t M, int64_t N, int64_t P, int64_t top_k,
-                                      void* workspace, size_t workspace_bytes,
-                                      w4a8_stream_t stream) {
-    using namespace w4a8;
+namespace w4a8 {
+namespace {
+
+template <typename InT>
+int gather_reduce_entry(const void* out2, const int32_t* sorted_token_ids,
+                        const float* topk_weights, const int32_t* num_tokens_post_padded,
+                        float* out, int64_t M, int64_t N, int64_t P, int64_t top_k,
+                        void* workspace, size_t workspace_bytes, w4a8_stream_t stream) {
     if (M < 0 || N <= 0 || P < 0 || top_k <= 0) return set_error("gather_reduce: bad sizes");
     if (M * top_k > INT32_MAX) return set_error("gather_reduce: size overflow");
     if (M == 0) return W4A8_OK;
@@ -167,8 +179,33 @@ extern "C" int w4a8_moe_gather_reduce(const void* out2, const int32_t* sorted_to
             sorted_token_ids, num_tokens_post_padded, map, P, M * top_k);
         if (int rc = launch_status()) return rc;
     }
-    return launch_gather_reduce(static_cast<const __half*>(out2), map, topk_weights, out, false, M,
-                                N, (int)top_k, st);
+    return launch_reduce(static_cast<const InT*>(out2), map, topk_weights, out, M, N, (int)top_k,
+                         st);
+}
+
+}  // namespace
+}  // namespace w4a8
+
+extern "C" int w4a8_moe_gather_reduce(const void* out2, const int32_t* sorted_token_ids,
+                                      const float* topk_weights,
+                                      const int32_t* num_tokens_post_padded, float* out,
+                                      int64_t M, int64_t N, int64_t P, int64_t top_k,
+                                      void* workspace, size_t workspace_bytes,
+                                      w4a8_stream_t stream) {
+    return w4a8::gather_reduce_entry<__half>(out2, sorted_token_ids, topk_weights,
+                                             num_tokens_post_padded, out, M, N, P, top_k,
+                                             workspace, workspace_bytes, stream);
+}
+
+extern "C" int w4a8_moe_gather_reduce_bf16(const void* out2, const int32_t* sorted_token_ids,
+                                           const float* topk_weights,
+                                           const int32_t* num_tokens_post_padded, float* out,
+                                           int64_t M, int64_t N, int64_t P, int64_t top_k,
+                                           void* workspace, size_t workspace_bytes,
+                                           w4a8_stream_t stream) {
+    return w4a8::gather_reduce_entry<__nv_bfloat16>(out2, sorted_token_ids, topk_weights,
+                                                    num_tokens_post_padded, out, M, N, P, top_k,
+                                                    workspace, workspace_bytes, stream);
 }
 
 namespace w4a8 {

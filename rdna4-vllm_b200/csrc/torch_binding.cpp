@@ -224,8 +224,9 @@ at::Tensor mmq_fp8_moe_gather_reduce_forward(const at::Tensor& out2,
                                              const at::Tensor& sorted_token_ids,
                                              const at::Tensor& topk_weights,
                                              const at::Tensor& ntp, int64_t top_k) {
-    TORCH_CHECK(out2.is_cuda() && out2.scalar_type() == at::kHalf && out2.dim() == 2,
-                "out2 must be (P,N) fp16 CUDA");
+    const bool bf16 = out2.scalar_type() == at::kBFloat16;
+    TORCH_CHECK(out2.is_cuda() && (bf16 || out2.scalar_type() == at::kHalf) && out2.dim() == 2,
+                "out2 must be (P,N) fp16 or bf16 CUDA");
     TORCH_CHECK(sorted_token_ids.scalar_type() == at::kInt && ntp.scalar_type() == at::kInt,
                 "sorted_token_ids / num_tokens_post_padded must be int32");
     TORCH_CHECK(topk_weights.scalar_type() == at::kFloat, "topk_weights must be fp32");
@@ -240,10 +241,11 @@ at::Tensor mmq_fp8_moe_gather_reduce_forward(const at::Tensor& out2,
     const c10::cuda::CUDAGuard guard(out2.device());
     auto out = at::empty({M, N}, out2.options().dtype(at::kFloat));
     auto ws = workspace(out2, w4a8_moe_gather_reduce_workspace_size(M, top_k));
-    check_status(w4a8_moe_gather_reduce(out2.data_ptr(), sorted_token_ids.data_ptr<int32_t>(),
-                                        topk_weights.data_ptr<float>(), ntp.data_ptr<int32_t>(),
-                                        out.data_ptr<float>(), M, N, sorted_token_ids.size(0),
-                                        top_k, ws.data_ptr(), (size_t)ws.numel(), cur_stream()),
+    const auto reduce = bf16 ? w4a8_moe_gather_reduce_bf16 : w4a8_moe_gather_reduce;
+    check_status(reduce(out2.data_ptr(), sorted_token_ids.data_ptr<int32_t>(),
+                        topk_weights.data_ptr<float>(), ntp.data_ptr<int32_t>(),
+                        out.data_ptr<float>(), M, N, sorted_token_ids.size(0), top_k,
+                        ws.data_ptr(), (size_t)ws.numel(), cur_stream()),
                  "mmq_fp8_moe_gather_reduce");
     return out;
 }
@@ -486,6 +488,184 @@ at::Tensor moe_decode_forward(const at::Tensor& x, const at::Tensor& w13, const 
     return out;
 }
 
+// ---- Block-scaled FP8 ----
+
+constexpr int64_t kScaleBlock = 128;
+
+int32_t dtype_code(at::ScalarType t, const char* what) {
+    if (t == at::kFloat) return 0;
+    if (t == at::kHalf) return 1;
+    if (t == at::kBFloat16) return 2;
+    TORCH_CHECK(false, what, " must be fp32, fp16 or bf16");
+}
+
+int64_t scale_blocks(int64_t n) { return (n + kScaleBlock - 1) / kScaleBlock; }
+
+bool is_e4m3(const at::Tensor& t) {
+    return t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kByte;
+}
+
+std::vector<at::Tensor> act_quant_fp8_block_forward(const at::Tensor& x) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(),
+                "x must be a contiguous (M, K) CUDA tensor");
+    const int32_t dt = dtype_code(x.scalar_type(), "x");
+    const int64_t M = x.size(0), K = x.size(1);
+    TORCH_CHECK(K > 0, "x must have at least one column");
+    const c10::cuda::CUDAGuard guard(x.device());
+    auto q = at::empty({M, K}, x.options().dtype(at::kFloat8_e4m3fn));
+    auto s = at::empty({M, scale_blocks(K)}, x.options().dtype(at::kFloat));
+    check_status(w4a8_act_quant_fp8_block(x.data_ptr(), dt, M, K, static_cast<uint8_t*>(q.data_ptr()),
+                                          s.data_ptr<float>(), cur_stream()),
+                 "act_quant_fp8_block");
+    return {q, s};
+}
+
+// Returns {q, scales, residual_out, normed}; an output that was not asked for is an empty tensor.
+std::vector<at::Tensor> rms_norm_quant_fp8_forward(const at::Tensor& x, const at::Tensor& weight,
+                                                   double eps,
+                                                   const c10::optional<at::Tensor>& residual,
+                                                   bool with_normed) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(),
+                "x must be a contiguous (M, H) CUDA tensor");
+    const int32_t dt = dtype_code(x.scalar_type(), "x");
+    const int64_t M = x.size(0), H = x.size(1);
+    TORCH_CHECK(H > 0, "x must have at least one column");
+    TORCH_CHECK(weight.device() == x.device() && weight.dim() == 1 && weight.size(0) == H &&
+                    weight.is_contiguous(),
+                "weight must be a contiguous (H,) tensor on x's device");
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
+                "weight must have x's type or fp32");
+    if (residual)
+        TORCH_CHECK(residual->device() == x.device() && residual->sizes() == x.sizes() &&
+                        residual->scalar_type() == x.scalar_type() && residual->is_contiguous(),
+                    "residual must be contiguous with x's shape, type and device");
+    const c10::cuda::CUDAGuard guard(x.device());
+    auto q = at::empty({M, H}, x.options().dtype(at::kFloat8_e4m3fn));
+    auto s = at::empty({M, scale_blocks(H)}, x.options().dtype(at::kFloat));
+    auto res = residual ? at::empty_like(x) : at::empty({0}, x.options());
+    auto nrm = with_normed ? at::empty_like(x) : at::empty({0}, x.options());
+    // an empty batch has no storage to point at; there is nothing to launch either
+    if (M > 0)
+        check_status(w4a8_rms_norm_quant_fp8(
+                         x.data_ptr(), residual ? residual->data_ptr() : nullptr,
+                         weight.data_ptr(), dt, dtype_code(weight.scalar_type(), "weight"),
+                         (float)eps, M, H, static_cast<uint8_t*>(q.data_ptr()),
+                         s.data_ptr<float>(), residual ? res.data_ptr() : nullptr,
+                         with_normed ? nrm.data_ptr() : nullptr, cur_stream()),
+                     "rms_norm_quant_fp8");
+    return {q, s, res, nrm};
+}
+
+void check_fp8_x(const at::Tensor& x, const at::Tensor& x_scales) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && is_e4m3(x) && x.is_contiguous(),
+                "x must be a contiguous (rows, K) e4m3 (float8_e4m3fn or uint8) CUDA tensor");
+    TORCH_CHECK(x.size(1) > 0, "x must have at least one column");
+    TORCH_CHECK(x_scales.device() == x.device() && x_scales.scalar_type() == at::kFloat &&
+                    x_scales.dim() == 2 && x_scales.size(0) == x.size(0) &&
+                    x_scales.size(1) == scale_blocks(x.size(1)) && x_scales.is_contiguous(),
+                "x_scales must be contiguous fp32 (rows, ceil(K/128)) on x's device");
+}
+
+at::Tensor fp8_block_gemm_forward(const at::Tensor& x, const at::Tensor& x_scales,
+                                  const at::Tensor& w, const at::Tensor& w_scales,
+                                  at::ScalarType out_dtype) {
+    check_fp8_x(x, x_scales);
+    const int64_t M = x.size(0), K = x.size(1);
+    TORCH_CHECK(w.device() == x.device() && w.dim() == 2 && is_e4m3(w) && w.is_contiguous() &&
+                    w.size(1) == K && w.size(0) > 0,
+                "w must be a contiguous (N, K) e4m3 tensor on x's device, K=", K);
+    const int64_t N = w.size(0);
+    TORCH_CHECK(w_scales.device() == x.device() && w_scales.scalar_type() == at::kFloat &&
+                    w_scales.dim() == 2 && w_scales.size(0) == scale_blocks(N) &&
+                    w_scales.size(1) == scale_blocks(K) && w_scales.is_contiguous(),
+                "w_scales must be contiguous fp32 (ceil(N/128), ceil(K/128)) on x's device");
+    const int32_t dt = dtype_code(out_dtype, "out_dtype");
+    const c10::cuda::CUDAGuard guard(x.device());
+    auto out = at::empty({M, N}, x.options().dtype(out_dtype));
+    check_status(w4a8_fp8_block_gemm(static_cast<const uint8_t*>(x.data_ptr()),
+                                     x_scales.data_ptr<float>(),
+                                     static_cast<const uint8_t*>(w.data_ptr()),
+                                     w_scales.data_ptr<float>(), out.data_ptr(), dt, M, N, K,
+                                     cur_stream()),
+                 "fp8_block_gemm");
+    return out;
+}
+
+void check_fp8_moe(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& w,
+                   const at::Tensor& w_scales,
+                   const c10::optional<at::Tensor>& sorted_token_ids,
+                   const at::Tensor& expert_ids, const at::Tensor& ntp, int64_t top_k,
+                   int64_t block_m) {
+    check_fp8_x(x, x_scales);
+    const int64_t K = x.size(1);
+    TORCH_CHECK(w.device() == x.device() && w.dim() == 3 && is_e4m3(w) && w.is_contiguous() &&
+                    w.size(2) == K && w.size(0) > 0 && w.size(1) > 0,
+                "w must be a contiguous (E, N, K) e4m3 tensor on x's device, K=", K);
+    TORCH_CHECK(w_scales.device() == x.device() && w_scales.scalar_type() == at::kFloat &&
+                    w_scales.dim() == 3 && w_scales.size(0) == w.size(0) &&
+                    w_scales.size(1) == scale_blocks(w.size(1)) &&
+                    w_scales.size(2) == scale_blocks(K) && w_scales.is_contiguous(),
+                "w_scales must be contiguous fp32 (E, ceil(N/128), ceil(K/128)) on x's device");
+    TORCH_CHECK(expert_ids.device() == x.device() && expert_ids.scalar_type() == at::kInt &&
+                    expert_ids.dim() == 1 && expert_ids.is_contiguous() &&
+                    ntp.device() == x.device() && ntp.scalar_type() == at::kInt &&
+                    ntp.numel() >= 1,
+                "expert_ids (P/block_m,) and num_tokens_post_padded (1,) must be contiguous int32 "
+                "on x's device");
+    TORCH_CHECK(top_k > 0 && block_m > 0, "top_k and block_m must be positive");
+    if (sorted_token_ids)
+        TORCH_CHECK(sorted_token_ids->device() == x.device() &&
+                        sorted_token_ids->scalar_type() == at::kInt &&
+                        sorted_token_ids->dim() == 1 && sorted_token_ids->is_contiguous(),
+                    "sorted_token_ids must be contiguous int32 (P,) on x's device");
+    const int64_t P = sorted_token_ids ? sorted_token_ids->size(0) : x.size(0);
+    TORCH_CHECK(P % block_m == 0 && expert_ids.size(0) == P / block_m, "expert_ids must have P/block_m=",
+                P / block_m, " entries and P=", P, " be a multiple of block_m");
+}
+
+at::Tensor fp8_block_moe_gemm_forward(const at::Tensor& x, const at::Tensor& x_scales,
+                                      const at::Tensor& w, const at::Tensor& w_scales,
+                                      const c10::optional<at::Tensor>& sorted_token_ids,
+                                      const at::Tensor& expert_ids, const at::Tensor& ntp,
+                                      int64_t top_k, int64_t block_m, at::ScalarType out_dtype) {
+    check_fp8_moe(x, x_scales, w, w_scales, sorted_token_ids, expert_ids, ntp, top_k, block_m);
+    const int64_t P = sorted_token_ids ? sorted_token_ids->size(0) : x.size(0);
+    const int32_t dt = dtype_code(out_dtype, "out_dtype");
+    const c10::cuda::CUDAGuard guard(x.device());
+    auto out = at::empty({P, w.size(1)}, x.options().dtype(out_dtype));
+    check_status(w4a8_fp8_block_moe_gemm(
+                     static_cast<const uint8_t*>(x.data_ptr()), x_scales.data_ptr<float>(),
+                     static_cast<const uint8_t*>(w.data_ptr()), w_scales.data_ptr<float>(),
+                     sorted_token_ids ? sorted_token_ids->data_ptr<int32_t>() : nullptr,
+                     expert_ids.data_ptr<int32_t>(), ntp.data_ptr<int32_t>(), out.data_ptr(), dt,
+                     x.size(0), w.size(0), w.size(1), x.size(1), P, top_k, block_m, cur_stream()),
+                 "fp8_block_moe_gemm");
+    return out;
+}
+
+std::vector<at::Tensor> fp8_block_moe_gemm1_silu_forward(
+    const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& w,
+    const at::Tensor& w_scales, const c10::optional<at::Tensor>& sorted_token_ids,
+    const at::Tensor& expert_ids, const at::Tensor& ntp, int64_t top_k, int64_t block_m) {
+    check_fp8_moe(x, x_scales, w, w_scales, sorted_token_ids, expert_ids, ntp, top_k, block_m);
+    TORCH_CHECK(w.size(1) % (2 * kScaleBlock) == 0,
+                "w must be (E, 2*inter, K) with inter a multiple of 128");
+    const int64_t P = sorted_token_ids ? sorted_token_ids->size(0) : x.size(0);
+    const int64_t inter = w.size(1) / 2;
+    const c10::cuda::CUDAGuard guard(x.device());
+    auto q = at::empty({P, inter}, x.options().dtype(at::kFloat8_e4m3fn));
+    auto s = at::empty({P, inter / kScaleBlock}, x.options().dtype(at::kFloat));
+    check_status(w4a8_fp8_block_moe_gemm1_silu(
+                     static_cast<const uint8_t*>(x.data_ptr()), x_scales.data_ptr<float>(),
+                     static_cast<const uint8_t*>(w.data_ptr()), w_scales.data_ptr<float>(),
+                     sorted_token_ids ? sorted_token_ids->data_ptr<int32_t>() : nullptr,
+                     expert_ids.data_ptr<int32_t>(), ntp.data_ptr<int32_t>(),
+                     static_cast<uint8_t*>(q.data_ptr()), s.data_ptr<float>(), x.size(0),
+                     w.size(0), inter, x.size(1), P, top_k, block_m, cur_stream()),
+                 "fp8_block_moe_gemm1_silu");
+    return {q, s};
+}
+
 }  // namespace
 
 // pt2_compliant_tag on every op, as the reference registers them (bindings.cpp:388-413); the
@@ -549,6 +729,18 @@ TORCH_LIBRARY(w4a8_b200, m) {
           "int top_k, int block_m, int kernel, bool weight_is_e2m1=False) -> Tensor");
     m.def("moe_align_block_size(Tensor topk_ids, int block_m, int num_experts, "
           "Tensor? expert_map=None, int num_local_experts=0) -> Tensor[]");
+    // Block-scaled FP8: activations with a scale per 128 columns, weights per 128 x 128 block.
+    m.def("act_quant_fp8_block(Tensor x) -> Tensor[]");
+    m.def("rms_norm_quant_fp8(Tensor x, Tensor weight, float eps, Tensor? residual, "
+          "bool with_normed) -> Tensor[]");
+    m.def("fp8_block_gemm(Tensor x, Tensor x_scales, Tensor w, Tensor w_scales, "
+          "ScalarType out_dtype) -> Tensor");
+    m.def("fp8_block_moe_gemm(Tensor x, Tensor x_scales, Tensor w, Tensor w_scales, "
+          "Tensor? sorted_token_ids, Tensor expert_ids, Tensor num_tokens_post_padded, int top_k, "
+          "int block_m, ScalarType out_dtype) -> Tensor");
+    m.def("fp8_block_moe_gemm1_silu(Tensor x, Tensor x_scales, Tensor w, Tensor w_scales, "
+          "Tensor? sorted_token_ids, Tensor expert_ids, Tensor num_tokens_post_padded, int top_k, "
+          "int block_m) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(w4a8_b200, CUDA, m) {
@@ -563,4 +755,9 @@ TORCH_LIBRARY_IMPL(w4a8_b200, CUDA, m) {
     m.impl("moe_decode_packed", &moe_decode_packed_forward);
     m.impl("moe_gemm1_silu", &gemm1_silu_impl);
     m.impl("moe_align_block_size", &moe_align_block_size_forward);
+    m.impl("act_quant_fp8_block", &act_quant_fp8_block_forward);
+    m.impl("rms_norm_quant_fp8", &rms_norm_quant_fp8_forward);
+    m.impl("fp8_block_gemm", &fp8_block_gemm_forward);
+    m.impl("fp8_block_moe_gemm", &fp8_block_moe_gemm_forward);
+    m.impl("fp8_block_moe_gemm1_silu", &fp8_block_moe_gemm1_silu_forward);
 }

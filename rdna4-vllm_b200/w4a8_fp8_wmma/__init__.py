@@ -129,7 +129,7 @@ def mmq_fp8_moe_gemm_scatter(x, w_packed, scales, sorted_token_ids, expert_ids,
 
 def mmq_fp8_moe_gather_reduce(out2, sorted_token_ids, topk_weights, num_tokens_post_padded,
                               top_k):
-    """Topk-weighted gather-reduce: (P, N) fp16 rows -> (M, N) fp32, M = numel(w) // top_k."""
+    """Topk-weighted gather-reduce: (P, N) fp16 or bf16 rows -> (M, N) fp32, M = numel(w) // top_k."""
     return torch.ops.w4a8_fp8_wmma.mmq_fp8_moe_gather_reduce(
         out2, sorted_token_ids, topk_weights, num_tokens_post_padded, top_k)
 
@@ -173,6 +173,72 @@ def route_topk(logits: torch.Tensor, top_k: int, renormalize: bool = True):
     ids, w, counts = torch.ops.w4a8_b200.route_topk(logits.contiguous(), int(top_k),
                                                     bool(renormalize))
     return ids, w, counts
+
+
+# ---- Block-scaled FP8: the layers that a mixed checkpoint keeps in 8 bits ----
+# e4m3 values (float8_e4m3fn, or their uint8 bytes) with one fp32 scale per 128 columns of an
+# activation row and per 128 x 128 block of a weight; the last block of a side may be short.
+
+def act_quant_fp8_block(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(M, K) fp16/bf16/fp32 -> (q (M, K) float8_e4m3fn, scales (M, ceil(K/128)) fp32): the rule
+    of act_quant_fp8 applied to each 128 columns of a row."""
+    q, s = torch.ops.w4a8_b200.act_quant_fp8_block(x.contiguous())
+    return q, s
+
+
+def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                       residual: torch.Tensor | None = None, with_normed: bool = False):
+    """RMS norm with the residual's addition and a block-scaled e4m3 output, in one pass.
+
+    h = x + residual (rounded to x's type; h = x without one), y = h * rsqrt(mean(h^2) + eps) *
+    weight in fp32. Returns (q (M, H) float8_e4m3fn, scales (M, ceil(H/128)) fp32, h as the new
+    residual or None, y in x's type if with_normed else None). x and residual fp16, bf16 or
+    fp32; weight in x's type or fp32.
+    """
+    q, s, res, normed = torch.ops.w4a8_b200.rms_norm_quant_fp8(
+        x.contiguous(), weight.contiguous(), float(eps),
+        residual.contiguous() if residual is not None else None, bool(with_normed))
+    return q, s, (res if residual is not None else None), (normed if with_normed else None)
+
+
+def fp8_block_gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor,
+                   w_scales: torch.Tensor, out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """Dense block-scaled FP8 GEMM: (M, K) e4m3 x (N, K) e4m3 -> (M, N) fp16, bf16 or fp32.
+
+    x_scales (M, ceil(K/128)), w_scales (ceil(N/128), ceil(K/128)), fp32. Sums are held in fp32
+    and rounded once. K a multiple of 16 takes the tensor cores; any other K is served by a
+    plain kernel.
+    """
+    return torch.ops.w4a8_b200.fp8_block_gemm(x, x_scales, w, w_scales, out_dtype)
+
+
+def fp8_block_moe_gemm(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
+                       num_tokens_post_padded, top_k: int, block_m: int,
+                       out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """Grouped block-scaled FP8 GEMM: out[r] = x[sorted_token_ids[r] // top_k] @ W[expert(r)]^T.
+
+    x (T, K) e4m3, w (E, N, K) e4m3, w_scales (E, ceil(N/128), ceil(K/128)); routing tensors in
+    the moe_align_block_size layout, block_m 16, 32, 64 or a multiple of 128. sorted_token_ids
+    None: x has P rows that are already in sorted order. Returns (P, N); padding rows and rows of
+    an expert id outside [0, E) are zero, rows past num_tokens_post_padded are not written.
+    """
+    return torch.ops.w4a8_b200.fp8_block_moe_gemm(
+        x, x_scales, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded,
+        int(top_k), int(block_m), out_dtype)
+
+
+def fp8_block_moe_gemm1_silu(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
+                             num_tokens_post_padded, top_k: int, block_m: int):
+    """Grouped gate_up GEMM + silu_and_mul + block quantisation: w (E, 2*inter, K) = [gate | up].
+
+    Returns (q (P, inter) float8_e4m3fn, scales (P, inter/128) fp32), what fp8_block_moe_gemm
+    reads for the down product. silu(gate) * up is evaluated in fp32 and rounded once, to e4m3.
+    inter must be a multiple of 128; the rest as fp8_block_moe_gemm.
+    """
+    q, s = torch.ops.w4a8_b200.fp8_block_moe_gemm1_silu(
+        x, x_scales, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded,
+        int(top_k), int(block_m))
+    return q, s
 
 
 # ---- Fake / meta impls (output contracts of the CUDA impls, reference __init__.py:240-297) ----
@@ -229,3 +295,38 @@ if _register_fake is not None:
                                         num_tokens_post_padded, top_k):
         return out2.new_empty((topk_weights.shape[0] // top_k, out2.shape[1]),
                               dtype=torch.float32)
+
+    def _blocks(n):
+        return (n + 127) // 128
+
+    @_register_fake("w4a8_b200::act_quant_fp8_block")
+    def _fake_act_quant_fp8_block(x):
+        M, K = x.shape
+        return [x.new_empty((M, K), dtype=torch.float8_e4m3fn),
+                x.new_empty((M, _blocks(K)), dtype=torch.float32)]
+
+    @_register_fake("w4a8_b200::rms_norm_quant_fp8")
+    def _fake_rms_norm_quant_fp8(x, weight, eps, residual, with_normed):
+        M, H = x.shape
+        return [x.new_empty((M, H), dtype=torch.float8_e4m3fn),
+                x.new_empty((M, _blocks(H)), dtype=torch.float32),
+                x.new_empty((M, H) if residual is not None else (0,)),
+                x.new_empty((M, H) if with_normed else (0,))]
+
+    @_register_fake("w4a8_b200::fp8_block_gemm")
+    def _fake_fp8_block_gemm(x, x_scales, w, w_scales, out_dtype):
+        return x.new_empty((x.shape[0], w.shape[0]), dtype=out_dtype)
+
+    @_register_fake("w4a8_b200::fp8_block_moe_gemm")
+    def _fake_fp8_block_moe_gemm(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
+                                 num_tokens_post_padded, top_k, block_m, out_dtype):
+        P = (x if sorted_token_ids is None else sorted_token_ids).shape[0]
+        return x.new_empty((P, w.shape[1]), dtype=out_dtype)
+
+    @_register_fake("w4a8_b200::fp8_block_moe_gemm1_silu")
+    def _fake_fp8_block_moe_gemm1_silu(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
+                                       num_tokens_post_padded, top_k, block_m):
+        P = (x if sorted_token_ids is None else sorted_token_ids).shape[0]
+        inter = w.shape[1] // 2
+        return [x.new_empty((P, inter), dtype=torch.float8_e4m3fn),
+                x.new_empty((P, _blocks(inter)), dtype=torch.float32)]
