@@ -122,7 +122,11 @@ int launch_fp8_simple(const Fp8Args& a, cudaStream_t st) {
 
 namespace {
 
-int run_fp8(const Fp8Args& a, cudaStream_t st) { return launch_fp8_simple(a, st); }
+// TMA needs rows of a multiple of 16 bytes from a 16-byte boundary; everything else takes the
+// plain kernel.
+int run_fp8(const Fp8Args& a, cudaStream_t st) {
+    return fp8_tc_ok(a) ? launch_fp8_tc(a, st) : launch_fp8_simple(a, st);
+}
 
 // Sizes and routing checks of the two grouped entries; 0 or W4A8_ERR_INVALID.
 int check_grouped(const std::string& o, const Fp8Args& a, int64_t top_k, int64_t block_m) {

@@ -1,0 +1,622 @@
+// gemm_fp8_tc.cu — block-scaled FP8 products on the 5th-generation tensor cores.
+//
+// A tile is up to 128 activation rows (the MMA's M side: row = tensor-memory lane) times BN weight
+// rows (its N side). Per 128-wide block g of K the tensor core returns acc = x_g w_g^T, and the
+// fold adds it to fp32 registers with one scalar per thread,
+//     tot[n] += (xs[row, g] * ws[n / 128, g]) * acc[n],
+// because a thread owns one row and the columns of one weight-scale block (two for the SiLU form,
+// gate and up). Tokens sit on the M side even when there are few: the weight rows, which are what
+// has to be read, still pass at the MMA's full N rate, and rows that do not exist are not loaded,
+// folded or stored.
+//
+// One persistent CTA per SM, 10 warps:
+//   warp 0     TMA producer: per stage one 128-byte column slab of the tile's x rows (a 2D box, or
+//              tile::gather4 through the routing, one 4-row gather per lane) and BN weight rows,
+//              in the 128-byte swizzle that the MMA's K-major descriptors read.
+//   warp 1     owns tensor memory; one thread issues 4 x tcgen05.mma.kind::f8f6f4 (K = 32) per
+//              block into a ring of fp32 accumulators (512 / BN of them).
+//   warps 2-9  fold: lane quarter warp % 4, one half of the columns each; then the epilogue.
+//
+// When there are fewer tiles than SMs, a cluster of S CTAs shares a tile: each takes a slice of
+// the K blocks, parks its fp32 partial tile in shared memory, and after a cluster barrier CTA r
+// sums rows r, r + S, ... over the cluster in rank order (distributed shared memory), so the
+// result does not depend on timing.
+//
+// Every mbarrier wait is bounded (sm100.cuh). When one gives up, the CTA stops waiting, waits
+// (boundedly) for its own copies in flight, writes NaN to the tile's outputs and frees tensor
+// memory.
+#include <cuda_bf16.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "fp8_block.h"
+#include "internal.h"
+#include "sm100.cuh"
+#include "tcgen05.cuh"
+
+namespace w4a8 {
+
+namespace {
+
+constexpr int kBlk = 128;
+constexpr int kThreads = 320;
+constexpr int kFoldWarps = 8;
+constexpr int kMaxSplit = 8;
+
+template <int BN>
+struct Cfg {
+    static constexpr int kStages = BN == 256 ? 4 : 6;
+    static constexpr int kAcc = 512 / BN;
+    static constexpr int kCols = BN / 2;            // columns per fold thread
+    static constexpr uint32_t kABytes = 128 * 128;  // a stage's x slab
+    static constexpr uint32_t kBBytes = BN * 128;
+    static constexpr int kPitch = BN + 4;           // floats per row of a parked partial tile
+};
+
+template <int BN>
+struct Smem {
+    uint8_t ring[Cfg<BN>::kStages][Cfg<BN>::kABytes + Cfg<BN>::kBBytes];  // 1024-byte aligned
+    // per warp: 32 rows x 128 bytes of finished outputs; the SiLU form keeps the row maxima of
+    // its two column halves here, [tile parity][half][row]
+    uint8_t stage_out[kFoldWarps][4096];
+    uint64_t full[Cfg<BN>::kStages], empty[Cfg<BN>::kStages];
+    uint64_t tfull[Cfg<BN>::kAcc], tempty[Cfg<BN>::kAcc];
+    uint32_t tmem_base;
+    int bad;
+};
+static_assert(sizeof(Smem<256>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(sizeof(Smem<128>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(128 * Cfg<256>::kPitch * 4 <= sizeof(Smem<256>::ring), "partial tile fits the ring");
+static_assert(128 * Cfg<128>::kPitch * 4 <= sizeof(Smem<128>::ring), "partial tile fits the ring");
+
+struct TcArgs {
+    Fp8Args f;
+    int tile_rows;  // 16, 32, 64 or 128 rows of x per tile
+    int split;      // CTAs per cluster
+    int n_tiles;    // weight tiles per row block
+};
+
+template <int N>
+struct Ring {
+    uint32_t idx = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++idx == N) {
+            idx = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// Tiles of one cluster: t = unit + i * units, t = row_block * n_tiles + n_tile.
+struct Walk {
+    int rb, nt, drb, dnt, n_tiles, blocks;
+    __device__ __forceinline__ Walk(int unit, int units, int n_tiles_, int blocks_)
+        : rb(unit / n_tiles_), nt(unit % n_tiles_), drb(units / n_tiles_), dnt(units % n_tiles_),
+          n_tiles(n_tiles_), blocks(blocks_) {}
+    __device__ __forceinline__ bool more() const { return rb < blocks; }
+    __device__ __forceinline__ void next() {
+        rb += drb;
+        nt += dnt;
+        if (nt >= n_tiles) {
+            nt -= n_tiles;
+            ++rb;
+        }
+    }
+};
+
+// x's row of output row r, or -1 when r is a row of zeros (absent expert e, padding slot).
+__device__ __forceinline__ int64_t source_row(const Fp8Args& a, int64_t r, int64_t rows, int e) {
+    if (r >= rows || e < 0 || e >= a.E) return -1;
+    if (!a.sorted_ids) return r;
+    const int slot = a.sorted_ids[r];
+    return slot >= 0 && slot < a.num_slots ? slot / a.top_k : -1;
+}
+
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x,
+                                            const int (&y)[4], uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
+        "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Waits for the loads into v; the operands keep every use of v behind the wait.
+__device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
+                   "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                   "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster(const float* p, uint32_t rank) {
+    uint32_t addr;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+
+__device__ __forceinline__ uint32_t pack2(int dtype, float a, float b) {
+    if (dtype == 1) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// `count` outputs of one row from column n on, held in 16 bytes (8 of 16 bits, 4 of fp32).
+__device__ __forceinline__ void store16(const Fp8Args& a, bool vec, int64_t r, int64_t n, uint4 v) {
+    const int size = a.out_dtype == 0 ? 4 : 2, per = 16 / size;
+    uint8_t* p = static_cast<uint8_t*>(a.out) + (r * a.N + n) * size;
+    if (vec && n + per <= a.N) {
+        *reinterpret_cast<uint4*>(p) = v;
+        return;
+    }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i >= per || n + i >= a.N) break;
+        if (size == 4) reinterpret_cast<uint32_t*>(p)[i] = w[i & 3];
+        else reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[(i >> 1) & 3] >> ((i & 1) * 16));
+    }
+}
+
+template <int BN, bool SILU, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
+              const __grid_constant__ CUtensorMap tmw) {
+    using C = Cfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    Smem<BN>& sm = *reinterpret_cast<Smem<BN>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    const Fp8Args& a = t.f;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* bad = &sm.bad;
+
+    const int S = SPLIT ? t.split : 1;
+    const int rank = SPLIT ? (int)cluster_rank() : 0;
+    const int64_t rows = a.ntp ? max((int64_t)0, min((int64_t)a.ntp[0], a.P)) : a.P;
+    const int blocks = (int)((rows + t.tile_rows - 1) / t.tile_rows);
+    const int per_expert = a.expert_ids ? a.block_m / t.tile_rows : 1;
+    const int G = (int)a.G;
+    const int g_lo = (int)((int64_t)G * rank / S), g_hi = (int)((int64_t)G * (rank + 1) / S);
+    const int live_warps = 2 * ((t.tile_rows + 31) / 32);  // fold warps whose lanes hold rows
+    const int n_step = SILU ? 128 : BN;                    // outputs per tile
+    const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
+    auto expert_of = [&](int rb) { return a.expert_ids ? a.expert_ids[rb / per_expert] : 0; };
+
+    if (tid == 0) {
+        sm.bad = 0;
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.empty[s], 1);
+        }
+        for (int s = 0; s < C::kAcc; ++s) {
+            mbar_init(&sm.tfull[s], 1);
+            mbar_init(&sm.tempty[s], live_warps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&sm.tmem_base)),
+                     "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::);
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::);
+    const uint32_t tmem = sm.tmem_base;
+
+    // One pass runs all of the CTA's tiles, every role at its own pace; with a split, one tile,
+    // and the cluster meets before the next.
+    Ring<C::kStages> st;  // stage ring position of the producer and of the MMA issuer
+    Ring<C::kAcc> tb;     // accumulator ring position of the MMA issuer and of the fold
+    uint32_t issued = 0;
+    Walk cur = first;
+    do {
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        const uint32_t stage_bytes = (uint32_t)t.tile_rows * 128 + C::kBBytes;
+        for (Walk w = cur; w.more(); w.next()) {
+            const int e = expert_of(w.rb);
+            if (e < 0 || e >= a.E) {
+                if (SPLIT) break;
+                continue;
+            }
+            const int r0 = w.rb * t.tile_rows;
+            int src[4] = {0, 0, 0, 0};  // gathered rows 4 * lane + i; padding rows read row 0
+            if (a.sorted_ids && 4 * lane < t.tile_rows)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    src[i] = (int)max((int64_t)0, source_row(a, r0 + 4 * lane + i, rows, e));
+            const int w_row = (int)(e * a.N) + w.nt * n_step;
+            for (int g = g_lo; g < g_hi; ++g) {
+                uint8_t* xa = sm.ring[st.idx];
+                uint64_t* fb = &sm.full[st.idx];
+                if (lane == 0) {
+                    mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
+                    mbar_expect_tx(fb, stage_bytes);
+                    uint8_t* wb = xa + C::kABytes;
+                    tma_load_2d(wb, &tmw, g * 128, w_row, fb);
+                    if (BN == 256)
+                        tma_load_2d(wb + 128 * 128, &tmw, g * 128,
+                                    SILU ? w_row + (int)(a.N / 2) : w_row + 128, fb);
+                    if (!a.sorted_ids) tma_load_2d(xa, &tmx, g * 128, r0, fb);
+                }
+                __syncwarp();
+                if (a.sorted_ids && 4 * lane < t.tile_rows)
+                    tma_gather4(xa + lane * 512, &tmx, g * 128, src, fb);
+                st.next();
+                ++issued;
+            }
+            if (SPLIT) break;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (lane == 0) {
+            constexpr uint32_t idesc = umma_idesc(128, BN);
+            for (Walk w = cur; w.more(); w.next()) {
+                const int e = expert_of(w.rb);
+                if (e < 0 || e >= a.E) {
+                    if (SPLIT) break;
+                    continue;
+                }
+                for (int g = g_lo; g < g_hi; ++g) {
+                    mbar_wait(&sm.full[st.idx], st.phase, bad);
+                    mbar_wait(&sm.tempty[tb.idx], tb.phase ^ 1, bad);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::);
+                    const uint32_t xa = smem_u32(sm.ring[st.idx]);
+                    const uint32_t d = tmem + tb.idx * BN;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t da = desc_sw128(xa + kk * 32);
+                        const uint64_t db = desc_sw128(xa + C::kABytes + kk * 32);
+                        asm volatile(
+                            "{\n\t.reg .pred p;\n\t"
+                            "setp.ne.b32 p, %4, 0;\n\t"
+                            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                            "l"(da), "l"(db), "r"(idesc), "r"(kk > 0 ? 1u : 0u));
+                    }
+                    asm volatile(
+                        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                        ::"r"(smem_u32(&sm.empty[st.idx])));
+                    asm volatile(
+                        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                        ::"r"(smem_u32(&sm.tfull[tb.idx])));
+                    st.next();
+                    tb.next();
+                }
+                if (SPLIT) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------- fold + epilogue ----------------
+        const int q = warp & 3, fw = warp - 2, half = fw >> 2;
+        const int row = q * 32 + lane;
+        if (q * 32 < t.tile_rows) {
+            // column of tot[j]: the plain form's half is contiguous; the SiLU form's holds 64
+            // gate columns, then the 64 matching up columns
+            auto col = [&](int j) {
+                return SILU ? (j < 64 ? half * 64 + j : 128 + half * 64 + j - 64) : half * C::kCols + j;
+            };
+            const int64_t NB = (a.N + kBlk - 1) / kBlk;
+            const bool vec = !SILU && (a.N * (a.out_dtype == 0 ? 4 : 2)) % 16 == 0 &&
+                             (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+            int done = 0;
+            for (Walk w = cur; w.more(); w.next()) {
+                const int e = expert_of(w.rb);
+                const bool present = e >= 0 && e < a.E;
+                const int64_t r0 = (int64_t)w.rb * t.tile_rows, r = r0 + row;
+                const int64_t src = row < t.tile_rows ? source_row(a, r, rows, e) : -1;
+                const int64_t n0 = (int64_t)w.nt * n_step;
+                float tot[C::kCols];
+#pragma unroll
+                for (int j = 0; j < C::kCols; ++j) tot[j] = 0.f;
+                if (present) {
+                    const float* xs = a.xs + max(src, (int64_t)0) * G;
+                    const int64_t b0 = SILU ? n0 / kBlk : min((n0 + half * C::kCols) / kBlk, NB - 1);
+                    const float* ws0 = a.ws + (e * NB + b0) * G;
+                    const float* ws1 = SILU ? ws0 + (a.N / 2 / kBlk) * G : ws0;
+                    float sx = g_lo < g_hi ? __ldg(xs + g_lo) : 0.f;
+                    float s0 = g_lo < g_hi ? __ldg(ws0 + g_lo) : 0.f;
+                    float s1 = SILU && g_lo < g_hi ? __ldg(ws1 + g_lo) : 0.f;
+                    for (int g = g_lo; g < g_hi; ++g) {
+                        const float f0 = sx * s0, f1 = SILU ? sx * s1 : f0;
+                        if (g + 1 < g_hi) {  // the next block's scales, behind this block's fold
+                            sx = __ldg(xs + g + 1);
+                            s0 = __ldg(ws0 + g + 1);
+                            if (SILU) s1 = __ldg(ws1 + g + 1);
+                        }
+                        mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::);
+                        const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + tb.idx * BN;
+                        uint32_t v[2][16];
+                        tmem_ld16_nowait(base + col(0), v[0]);
+                        tmem_wait16(v[0]);
+#pragma unroll
+                        for (int j = 0; j < C::kCols; j += 16) {
+                            uint32_t(&cur)[16] = v[(j / 16) & 1];
+                            uint32_t(&nxt)[16] = v[(j / 16 + 1) & 1];
+                            if (j + 16 < C::kCols) tmem_ld16_nowait(base + col(j + 16), nxt);
+                            const float f = j < C::kCols / 2 ? f0 : f1;
+                            const float2 f2 = make_float2(f, f);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const float2 p = ffma2(
+                                    make_float2(__uint_as_float(cur[i]), __uint_as_float(cur[i + 1])),
+                                    f2, make_float2(tot[j + i], tot[j + i + 1]));
+                                tot[j + i] = p.x;
+                                tot[j + i + 1] = p.y;
+                            }
+                            if (j + 16 < C::kCols) tmem_wait16(nxt);
+                        }
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.tempty[tb.idx]);
+                        tb.next();
+                    }
+                }
+                // rows of zeros stay zero whatever the lane's accumulator held
+                const float poison = *bad ? __int_as_float(0x7fffffff) : 0.f;
+#pragma unroll
+                for (int j = 0; j < C::kCols; ++j) tot[j] = src < 0 ? poison : tot[j] + poison;
+                if (SPLIT) {
+                    // park the partial tile; the ring is idle once the last accumulator was read
+                    if (row < t.tile_rows) {
+                        float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
+#pragma unroll
+                        for (int j = 0; j < C::kCols; j += 4)
+                            *reinterpret_cast<float4*>(part + col(j)) =
+                                make_float4(tot[j], tot[j + 1], tot[j + 2], tot[j + 3]);
+                    }
+                } else if (SILU) {
+                    float m = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) {
+                        tot[j] = silu_mul(tot[j], tot[(j + 64) % C::kCols]);
+                        m = fmaxf(m, fabsf(tot[j]));
+                    }
+                    // the row's other 64 outputs are with the warp of the other half
+                    float* amax = reinterpret_cast<float*>(sm.stage_out) + (done & 1) * 256;
+                    amax[half * 128 + row] = m;
+                    asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
+                    m = fmaxf(m, amax[(half ^ 1) * 128 + row]);
+                    const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
+                    const float rcp = __frcp_rn(s);
+                    if (row < t.tile_rows && r < rows) {
+                        const int64_t inter = a.N / 2;
+                        if (half == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
+                        uint32_t* qp = reinterpret_cast<uint32_t*>(a.q + r * inter + n0 + half * 64);
+#pragma unroll
+                        for (int j = 0; j < 64; j += 4)
+                            qp[j / 4] = (uint32_t)quant_pair(tot[j], tot[j + 1], s, rcp) |
+                                        (uint32_t)quant_pair(tot[j + 2], tot[j + 3], s, rcp) << 16;
+                    }
+                } else {
+                    // 128 bytes of each row at a time through the warp's staging area (16-byte
+                    // chunks swizzled by row), so that global stores cover whole lines
+                    uint8_t* so = sm.stage_out[fw];
+                    const int per = a.out_dtype == 0 ? 32 : 64;  // columns per pass
+#pragma unroll
+                    for (int c = 0; c < C::kCols; c += 32) {
+                        if (a.out_dtype == 0) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<float4*>(so + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                                    make_float4(tot[c + 4 * i], tot[c + 4 * i + 1],
+                                                tot[c + 4 * i + 2], tot[c + 4 * i + 3]);
+                        } else {
+                            const int i0 = (c & 32) ? 4 : 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                uint4 u;
+                                u.x = pack2(a.out_dtype, tot[c + 8 * i], tot[c + 8 * i + 1]);
+                                u.y = pack2(a.out_dtype, tot[c + 8 * i + 2], tot[c + 8 * i + 3]);
+                                u.z = pack2(a.out_dtype, tot[c + 8 * i + 4], tot[c + 8 * i + 5]);
+                                u.w = pack2(a.out_dtype, tot[c + 8 * i + 6], tot[c + 8 * i + 7]);
+                                *reinterpret_cast<uint4*>(so + lane * 128 + (((i0 + i) ^ (lane & 7)) << 4)) = u;
+                            }
+                            if (!(c & 32)) continue;  // the second half of the line follows
+                        }
+                        __syncwarp();
+                        const int64_t nc = n0 + col(c + 32 - per) + (lane & 7) * (per / 8);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int rr = i * 4 + (lane >> 3), tr = q * 32 + rr;
+                            const uint4 u = *reinterpret_cast<const uint4*>(
+                                so + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+                            if (tr < t.tile_rows && r0 + tr < rows && nc < a.N)
+                                store16(a, vec, r0 + tr, nc, u);
+                        }
+                        __syncwarp();
+                    }
+                }
+                ++done;
+                if (SPLIT) break;
+            }
+        }
+        __syncwarp();
+    }
+
+    if (SPLIT) {
+        // CTA `rank` finishes rows rank, rank + S, ... of the cluster's tile
+        cluster_sync();
+        if (warp >= 2 && cur.more()) {
+            const int64_t r0 = (int64_t)cur.rb * t.tile_rows, n0 = (int64_t)cur.nt * n_step;
+            const bool vec = !SILU && (a.N * (a.out_dtype == 0 ? 4 : 2)) % 16 == 0 &&
+                             (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+            const float* part = reinterpret_cast<const float*>(sm.ring);
+            for (int tr = rank + S * (warp - 2); tr < t.tile_rows; tr += S * kFoldWarps) {
+                const int64_t r = r0 + tr;
+                if (r >= rows) break;
+                float4 sum[BN / 128];
+#pragma unroll
+                for (int c = 0; c < BN / 128; ++c) {
+                    float4 v[kMaxSplit];
+#pragma unroll
+                    for (int k = 0; k < kMaxSplit; ++k)
+                        if (k < S) v[k] = ld_cluster(part + tr * C::kPitch + c * 128 + 4 * lane, k);
+                    sum[c] = v[0];
+#pragma unroll
+                    for (int k = 1; k < kMaxSplit; ++k)
+                        if (k < S) {
+                            sum[c].x += v[k].x;
+                            sum[c].y += v[k].y;
+                            sum[c].z += v[k].z;
+                            sum[c].w += v[k].w;
+                        }
+                }
+                if (SILU) {
+                    const float4 g4 = sum[0], u4 = sum[BN / 128 - 1];
+                    const float h[4] = {silu_mul(g4.x, u4.x), silu_mul(g4.y, u4.y),
+                                        silu_mul(g4.z, u4.z), silu_mul(g4.w, u4.w)};
+                    float m = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
+                    const float rcp = __frcp_rn(s);
+                    const int64_t inter = a.N / 2;
+                    if (lane == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
+                    *reinterpret_cast<uint32_t*>(a.q + r * inter + n0 + 4 * lane) =
+                        (uint32_t)quant_pair(h[0], h[1], s, rcp) |
+                        (uint32_t)quant_pair(h[2], h[3], s, rcp) << 16;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < BN / 128; ++c) {
+                        const int64_t n = n0 + c * 128 + 4 * lane;
+                        const float o[4] = {sum[c].x, sum[c].y, sum[c].z, sum[c].w};
+                        if (a.out_dtype == 0) {
+                            float* p = static_cast<float*>(a.out) + r * a.N + n;
+                            if (vec && n + 4 <= a.N) *reinterpret_cast<float4*>(p) = sum[c];
+                            else
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (n + i < a.N) p[i] = o[i];
+                        } else {
+                            uint16_t* p = static_cast<uint16_t*>(a.out) + r * a.N + n;
+                            const uint32_t lo = pack2(a.out_dtype, o[0], o[1]);
+                            const uint32_t hi = pack2(a.out_dtype, o[2], o[3]);
+                            if (vec && n + 4 <= a.N) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+                            else
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (n + i < a.N) p[i] = (uint16_t)((i < 2 ? lo : hi) >> ((i & 1) * 16));
+                        }
+                    }
+                }
+            }
+        }
+        // no CTA leaves, or loads its next tile over the parked one, while that is still read
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        cluster_sync();
+        cur.next();
+    }
+    } while (SPLIT && cur.more());
+    // after a wait that gave up: leave no copy in flight
+    if (tid == 0 && *bad) {
+        const uint64_t t0 = global_ns();
+        for (uint32_t j = 0; j < (uint32_t)C::kStages && j < issued; ++j)
+            while (!mbar_try(&sm.full[j], ((issued - 1 - j) / C::kStages) & 1) &&
+                   global_ns() - t0 < kWaitLimitNs) {
+            }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::);
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::);
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+int sm_count() {
+    int dev = 0, n = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n > 0 ? n : 148;
+}
+
+template <int BN, bool SILU, bool SPLIT>
+int launch_t(const TcArgs& t, int64_t tiles, cudaStream_t st) {
+    const Fp8Args& a = t.f;
+    CUtensorMap tmx, tmw;
+    if (!make_tma_map_u8(&tmx, a.x, (uint64_t)a.x_rows, (uint64_t)a.K, 128,
+                         a.sorted_ids ? 1 : t.tile_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !make_tma_map_u8(&tmw, a.w, (uint64_t)(a.E * a.N), (uint64_t)a.K, 128, 128,
+                         CU_TENSOR_MAP_SWIZZLE_128B))
+        return set_error("fp8_block: tensor map encoding failed");
+    auto kern = fp8_tc_kernel<BN, SILU, SPLIT>;
+    const int smem = (int)sizeof(Smem<BN>) + 1024;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, std::max(1, sm_count() / t.split)) * t.split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {(unsigned)t.split, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = SPLIT ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kern, t, tmx, tmw);
+    if (e != cudaSuccess) return (int)e;
+    return launch_status();
+}
+
+}  // namespace
+
+bool fp8_tc_ok(const Fp8Args& a) {
+    return a.K % 16 == 0 && a.x_rows > 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 &&
+           (reinterpret_cast<uintptr_t>(a.w) & 15) == 0 &&
+           (!a.silu || (reinterpret_cast<uintptr_t>(a.q) & 3) == 0);
+}
+
+int launch_fp8_tc(const Fp8Args& a, cudaStream_t st) {
+    TcArgs t{};
+    t.f = a;
+    const int64_t rows = a.expert_ids ? a.block_m : a.P;
+    t.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    // row blocks that can hold work: with routing, at most one per slot
+    int64_t blocks = (a.P + t.tile_rows - 1) / t.tile_rows;
+    if (a.sorted_ids) blocks = std::min<int64_t>(blocks, (int64_t)a.num_slots * std::max(1, a.block_m / t.tile_rows));
+    const int sms = sm_count();
+    const int64_t n = a.silu ? a.N / 2 : a.N;
+    // Wide tiles once they fill the GPU; below that, narrow tiles and a cluster along K.
+    const int64_t wide = blocks * ((n + (a.silu ? 127 : 255)) / (a.silu ? 128 : 256));
+    const int64_t narrow = blocks * ((n + 127) / 128);
+    const bool bn256 = a.silu || wide >= sms;
+    const int64_t tiles = bn256 ? wide : narrow;
+    t.n_tiles = (int)(tiles / blocks);
+    t.split = 1;
+    while (t.split < kMaxSplit && tiles * t.split * 2 <= sms && a.G >= t.split * 4) t.split *= 2;
+    const bool split = t.split > 1;
+    if (a.silu)
+        return split ? launch_t<256, true, true>(t, tiles, st) : launch_t<256, true, false>(t, tiles, st);
+    if (bn256) return launch_t<256, false, false>(t, tiles, st);
+    return split ? launch_t<128, false, true>(t, tiles, st) : launch_t<128, false, false>(t, tiles, st);
+}
+
+}  // namespace w4a8
