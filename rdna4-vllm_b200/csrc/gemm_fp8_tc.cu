@@ -47,20 +47,21 @@ constexpr int kMaxSplit = 8;
 
 template <int BN>
 struct Cfg {
-    static constexpr int kStages = BN == 256 ? 4 : 6;
+    static constexpr int kStages = BN == 256 ? 3 : 6;
     static constexpr int kAcc = 512 / BN;
     static constexpr int kCols = BN / 2;            // columns per fold thread
     static constexpr uint32_t kABytes = 128 * 128;  // a stage's x slab
     static constexpr uint32_t kBBytes = BN * 128;
+    static constexpr int kLines = kCols / 64;       // staged 128-byte lines per warp and pass
     static constexpr int kPitch = BN + 4;           // floats per row of a parked partial tile
 };
 
 template <int BN>
 struct Smem {
     uint8_t ring[Cfg<BN>::kStages][Cfg<BN>::kABytes + Cfg<BN>::kBBytes];  // 1024-byte aligned
-    // per warp: 32 rows x 128 bytes of finished outputs; the SiLU form keeps the row maxima of
-    // its two column halves here, [tile parity][half][row]
-    uint8_t stage_out[kFoldWarps][4096];
+    // per warp: lines of 32 rows x 128 bytes of finished outputs (1024-byte aligned); the SiLU
+    // form keeps the row maxima of its two column halves here, [tile parity][half][row]
+    uint8_t stage_out[kFoldWarps][Cfg<BN>::kLines][4096];
     uint64_t full[Cfg<BN>::kStages], empty[Cfg<BN>::kStages];
     uint64_t tfull[Cfg<BN>::kAcc], tempty[Cfg<BN>::kAcc];
     uint32_t tmem_base;
@@ -76,6 +77,7 @@ struct TcArgs {
     int tile_rows;  // 16, 32, 64 or 128 rows of x per tile
     int split;      // CTAs per cluster
     int n_tiles;    // weight tiles per row block
+    int out_tma;    // out's rows are TMA-storable: 16-byte aligned base and pitch
 };
 
 template <int N>
@@ -154,7 +156,11 @@ __device__ __forceinline__ float4 ld_cluster(const float* p, uint32_t rank) {
     return v;
 }
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+// silu(g) * u with the fast exponential and quotient, together within 10 units of 2^-24 plus
+// |g| 2^-24 from the exponential's argument: below the product sums' own error.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+    return __fdividef(g, 1.f + __expf(-g)) * u;
+}
 
 __device__ __forceinline__ uint32_t pack2(int dtype, float a, float b) {
     if (dtype == 1) {
@@ -165,7 +171,7 @@ __device__ __forceinline__ uint32_t pack2(int dtype, float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// `count` outputs of one row from column n on, held in 16 bytes (8 of 16 bits, 4 of fp32).
+// Outputs of one row from column n on, held in 16 bytes (8 of 16 bits, 4 of fp32).
 __device__ __forceinline__ void store16(const Fp8Args& a, bool vec, int64_t r, int64_t n, uint4 v) {
     const int size = a.out_dtype == 0 ? 4 : 2, per = 16 / size;
     uint8_t* p = static_cast<uint8_t*>(a.out) + (r * a.N + n) * size;
@@ -173,19 +179,61 @@ __device__ __forceinline__ void store16(const Fp8Args& a, bool vec, int64_t r, i
         *reinterpret_cast<uint4*>(p) = v;
         return;
     }
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (i >= per || n + i >= a.N) break;
-        if (size == 4) reinterpret_cast<uint32_t*>(p)[i] = w[i & 3];
-        else reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[(i >> 1) & 3] >> ((i & 1) * 16));
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(&v);
+#pragma unroll 1
+    for (int i = 0; i < (int)min((int64_t)per, a.N - n) * size / 2; ++i)
+        reinterpret_cast<uint16_t*>(p)[i] = h[i];
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(smem_u32(src))
+                 : "memory");
+}
+
+// Before a warp writes its staging area: its last TMA stores have read it.
+__device__ __forceinline__ void staging_free() {
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+}
+
+// Sends a warp's staged lines (32 rows x 128 bytes, 16-byte chunks XORed with row % 8, the
+// 128-byte swizzle) to rows r_first + [0, box_rows) and columns n_first on. `whole`: the box may
+// be stored as it is; else only rows below `rows` are, by plain stores.
+__device__ __forceinline__ void send_lines(const TcArgs& t, const CUtensorMap* tmo, uint8_t* so,
+                                           int lines, int64_t r_first, int64_t rows, int64_t n_first,
+                                           bool whole) {
+    const Fp8Args& a = t.f;
+    const int lane = threadIdx.x & 31;
+    const int size = a.out_dtype == 0 ? 4 : 2, per = 128 / size;
+    const int box_rows = min(t.tile_rows, 32);
+    if (t.out_tma && whole) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            for (int l = 0; l < lines; ++l)
+                if (n_first + l * per < a.N)
+                    tma_store_2d(tmo, (int)(n_first + l * per) * size, (int)r_first, so + l * 4096);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        return;
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < lines * 8; ++i) {
+        const int rr = (i & 7) * 4 + (lane >> 3), line = i >> 3;
+        const uint4 u = *reinterpret_cast<const uint4*>(so + line * 4096 + rr * 128 +
+                                                        (((lane & 7) ^ (rr & 7)) << 4));
+        const int64_t n = n_first + line * per + (lane & 7) * (per / 8);
+        if (rr < box_rows && r_first + rr < rows && n < a.N) store16(a, t.out_tma, r_first + rr, n, u);
     }
 }
 
 template <int BN, bool SILU, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
-              const __grid_constant__ CUtensorMap tmw) {
+              const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmo) {
     using C = Cfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     Smem<BN>& sm = *reinterpret_cast<Smem<BN>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -323,8 +371,6 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 return SILU ? (j < 64 ? half * 64 + j : 128 + half * 64 + j - 64) : half * C::kCols + j;
             };
             const int64_t NB = (a.N + kBlk - 1) / kBlk;
-            const bool vec = !SILU && (a.N * (a.out_dtype == 0 ? 4 : 2)) % 16 == 0 &&
-                             (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
             int done = 0;
             for (Walk w = cur; w.more(); w.next()) {
                 const int e = expert_of(w.rb);
@@ -409,54 +455,51 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     if (row < t.tile_rows && r < rows) {
                         const int64_t inter = a.N / 2;
                         if (half == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
-                        uint32_t* qp = reinterpret_cast<uint32_t*>(a.q + r * inter + n0 + half * 64);
+                        uint4* qp = reinterpret_cast<uint4*>(a.q + r * inter + n0 + half * 64);
 #pragma unroll
-                        for (int j = 0; j < 64; j += 4)
-                            qp[j / 4] = (uint32_t)quant_pair(tot[j], tot[j + 1], s, rcp) |
-                                        (uint32_t)quant_pair(tot[j + 2], tot[j + 3], s, rcp) << 16;
+                        for (int j = 0; j < 64; j += 16) {
+                            uint32_t u[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                u[i] = (uint32_t)quant_pair(tot[j + 4 * i], tot[j + 4 * i + 1], s, rcp) |
+                                       (uint32_t)quant_pair(tot[j + 4 * i + 2], tot[j + 4 * i + 3], s, rcp) << 16;
+                            qp[j / 16] = make_uint4(u[0], u[1], u[2], u[3]);
+                        }
                     }
                 } else {
-                    // 128 bytes of each row at a time through the warp's staging area (16-byte
-                    // chunks swizzled by row), so that global stores cover whole lines
-                    uint8_t* so = sm.stage_out[fw];
-                    const int per = a.out_dtype == 0 ? 32 : 64;  // columns per pass
+                    uint8_t* so = sm.stage_out[fw][0];
+                    const bool whole = !a.ntp || r0 + q * 32 + min(t.tile_rows, 32) <= rows;
+                    if (a.out_dtype == 0) {
 #pragma unroll
-                    for (int c = 0; c < C::kCols; c += 32) {
-                        if (a.out_dtype == 0) {
+                        for (int c0 = 0; c0 < C::kCols; c0 += C::kCols / 2) {  // 32 columns a line
+                            staging_free();
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                *reinterpret_cast<float4*>(so + lane * 128 + ((i ^ (lane & 7)) << 4)) =
-                                    make_float4(tot[c + 4 * i], tot[c + 4 * i + 1],
-                                                tot[c + 4 * i + 2], tot[c + 4 * i + 3]);
-                        } else {
-                            const int i0 = (c & 32) ? 4 : 0;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint4 u;
-                                u.x = pack2(a.out_dtype, tot[c + 8 * i], tot[c + 8 * i + 1]);
-                                u.y = pack2(a.out_dtype, tot[c + 8 * i + 2], tot[c + 8 * i + 3]);
-                                u.z = pack2(a.out_dtype, tot[c + 8 * i + 4], tot[c + 8 * i + 5]);
-                                u.w = pack2(a.out_dtype, tot[c + 8 * i + 6], tot[c + 8 * i + 7]);
-                                *reinterpret_cast<uint4*>(so + lane * 128 + (((i0 + i) ^ (lane & 7)) << 4)) = u;
-                            }
-                            if (!(c & 32)) continue;  // the second half of the line follows
+                            for (int c = 0; c < C::kCols / 2; c += 4)
+                                *reinterpret_cast<float4*>(so + (c / 32) * 4096 + lane * 128 +
+                                                           (((c / 4 % 8) ^ (lane & 7)) << 4)) =
+                                    make_float4(tot[c0 + c], tot[c0 + c + 1], tot[c0 + c + 2],
+                                                tot[c0 + c + 3]);
+                            send_lines(t, &tmo, so, C::kLines, r0 + q * 32, rows, n0 + col(c0), whole);
                         }
-                        __syncwarp();
-                        const int64_t nc = n0 + col(c + 32 - per) + (lane & 7) * (per / 8);
+                    } else {
+                        staging_free();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int rr = i * 4 + (lane >> 3), tr = q * 32 + rr;
-                            const uint4 u = *reinterpret_cast<const uint4*>(
-                                so + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-                            if (tr < t.tile_rows && r0 + tr < rows && nc < a.N)
-                                store16(a, vec, r0 + tr, nc, u);
+                        for (int c = 0; c < C::kCols; c += 8) {  // 64 columns a line
+                            uint4 u;
+                            u.x = pack2(a.out_dtype, tot[c], tot[c + 1]);
+                            u.y = pack2(a.out_dtype, tot[c + 2], tot[c + 3]);
+                            u.z = pack2(a.out_dtype, tot[c + 4], tot[c + 5]);
+                            u.w = pack2(a.out_dtype, tot[c + 6], tot[c + 7]);
+                            *reinterpret_cast<uint4*>(so + (c / 64) * 4096 + lane * 128 +
+                                                      (((c / 8 % 8) ^ (lane & 7)) << 4)) = u;
                         }
-                        __syncwarp();
+                        send_lines(t, &tmo, so, C::kLines, r0 + q * 32, rows, n0 + col(0), whole);
                     }
                 }
                 ++done;
                 if (SPLIT) break;
             }
+            if (!SILU && !SPLIT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
         __syncwarp();
     }
@@ -466,8 +509,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         cluster_sync();
         if (warp >= 2 && cur.more()) {
             const int64_t r0 = (int64_t)cur.rb * t.tile_rows, n0 = (int64_t)cur.nt * n_step;
-            const bool vec = !SILU && (a.N * (a.out_dtype == 0 ? 4 : 2)) % 16 == 0 &&
-                             (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+            const bool vec = t.out_tma;
             const float* part = reinterpret_cast<const float*>(sm.ring);
             for (int tr = rank + S * (warp - 2); tr < t.tile_rows; tr += S * kFoldWarps) {
                 const int64_t r = r0 + tr;
@@ -559,9 +601,15 @@ int sm_count() {
 }
 
 template <int BN, bool SILU, bool SPLIT>
-int launch_t(const TcArgs& t, int64_t tiles, cudaStream_t st) {
+int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
     const Fp8Args& a = t.f;
-    CUtensorMap tmx, tmw;
+    CUtensorMap tmx, tmw, tmo{};
+    const int64_t pitch = a.N * (a.out_dtype == 0 ? 4 : 2);
+    t.out_tma = !SILU && pitch % 16 == 0 && pitch <= INT32_MAX && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+    if (t.out_tma && !SPLIT &&
+        !make_tma_map_u8(&tmo, a.out, (uint64_t)a.P, (uint64_t)pitch, 128, std::min(t.tile_rows, 32),
+                         CU_TENSOR_MAP_SWIZZLE_128B))
+        return set_error("fp8_block: tensor map encoding failed");
     if (!make_tma_map_u8(&tmx, a.x, (uint64_t)a.x_rows, (uint64_t)a.K, 128,
                          a.sorted_ids ? 1 : t.tile_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !make_tma_map_u8(&tmw, a.w, (uint64_t)(a.E * a.N), (uint64_t)a.K, 128, 128,
@@ -581,7 +629,7 @@ int launch_t(const TcArgs& t, int64_t tiles, cudaStream_t st) {
     at[0].val.clusterDim = {(unsigned)t.split, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = SPLIT ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, t, tmx, tmw);
+    e = cudaLaunchKernelEx(&cfg, kern, t, tmx, tmw, tmo);
     if (e != cudaSuccess) return (int)e;
     return launch_status();
 }
@@ -591,7 +639,7 @@ int launch_t(const TcArgs& t, int64_t tiles, cudaStream_t st) {
 bool fp8_tc_ok(const Fp8Args& a) {
     return a.K % 16 == 0 && a.x_rows > 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 &&
            (reinterpret_cast<uintptr_t>(a.w) & 15) == 0 &&
-           (!a.silu || (reinterpret_cast<uintptr_t>(a.q) & 3) == 0);
+           (!a.silu || (reinterpret_cast<uintptr_t>(a.q) & 15) == 0);
 }
 
 int launch_fp8_tc(const Fp8Args& a, cudaStream_t st) {
