@@ -29,6 +29,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "fp8_block.h"
@@ -45,32 +46,38 @@ constexpr int kThreads = 320;
 constexpr int kFoldWarps = 8;
 constexpr int kMaxSplit = 8;
 
-template <int BN>
+// TR: rows a tile may have, 32 or 128. A short tile's stages hold only its rows; the MMA's
+// 128-row operand then runs on into the weight rows behind them, and those lanes are ignored.
+template <int BN, int TR>
 struct Cfg {
-    static constexpr int kStages = BN == 256 ? 3 : 6;
-    static constexpr int kAcc = 512 / BN;
-    static constexpr int kCols = BN / 2;            // columns per fold thread
-    static constexpr uint32_t kABytes = 128 * 128;  // a stage's x slab
+    static constexpr uint32_t kABytes = TR * 128;  // a stage's x slab
     static constexpr uint32_t kBBytes = BN * 128;
-    static constexpr int kLines = kCols / 64;       // staged 128-byte lines per warp and pass
-    static constexpr int kPitch = BN + 4;           // floats per row of a parked partial tile
+    static constexpr int kStages = TR == 32 ? (BN == 256 ? 5 : 10) : (BN == 256 ? 3 : 6);
+    static constexpr int kAcc = 512 / BN;
+    static constexpr int kCols = BN / 2;           // columns per fold thread
+    static constexpr int kLive = TR == 32 ? 2 : kFoldWarps;  // fold warps that may hold rows
+    static constexpr int kLines = kCols / 64;      // staged 128-byte lines per warp and pass
+    static constexpr int kPitch = BN + 4;          // floats per row of a parked partial tile
 };
 
-template <int BN>
+template <int BN, int TR>
 struct Smem {
-    uint8_t ring[Cfg<BN>::kStages][Cfg<BN>::kABytes + Cfg<BN>::kBBytes];  // 1024-byte aligned
+    using C = Cfg<BN, TR>;
+    uint8_t ring[C::kStages][C::kABytes + C::kBBytes];  // 1024-byte aligned
     // per warp: lines of 32 rows x 128 bytes of finished outputs (1024-byte aligned); the SiLU
     // form keeps the row maxima of its two column halves here, [tile parity][half][row]
-    uint8_t stage_out[kFoldWarps][Cfg<BN>::kLines][4096];
-    uint64_t full[Cfg<BN>::kStages], empty[Cfg<BN>::kStages];
-    uint64_t tfull[Cfg<BN>::kAcc], tempty[Cfg<BN>::kAcc];
+    uint8_t stage_out[C::kLive][C::kLines][4096];
+    uint64_t full[C::kStages], empty[C::kStages];
+    uint64_t tfull[C::kAcc], tempty[C::kAcc];
     uint32_t tmem_base;
     int bad;
+    static_assert(C::kABytes + C::kBBytes >= 128 * 128, "the x operand's reads stay in the ring");
+    static_assert(TR * C::kPitch * 4 <= sizeof(ring), "a partial tile fits the ring");
 };
-static_assert(sizeof(Smem<256>) + 1024 <= 227 * 1024, "shared memory");
-static_assert(sizeof(Smem<128>) + 1024 <= 227 * 1024, "shared memory");
-static_assert(128 * Cfg<256>::kPitch * 4 <= sizeof(Smem<256>::ring), "partial tile fits the ring");
-static_assert(128 * Cfg<128>::kPitch * 4 <= sizeof(Smem<128>::ring), "partial tile fits the ring");
+static_assert(sizeof(Smem<256, 128>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(sizeof(Smem<128, 128>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(sizeof(Smem<256, 32>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(sizeof(Smem<128, 32>) + 1024 <= 227 * 1024, "shared memory");
 
 struct TcArgs {
     Fp8Args f;
@@ -162,18 +169,23 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
     return __fdividef(g, 1.f + __expf(-g)) * u;
 }
 
-__device__ __forceinline__ uint32_t pack2(int dtype, float a, float b) {
-    if (dtype == 1) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Outputs of one row from column n on, held in 16 bytes (8 of 16 bits, 4 of fp32).
+template <int size>
 __device__ __forceinline__ void store16(const Fp8Args& a, bool vec, int64_t r, int64_t n, uint4 v) {
-    const int size = a.out_dtype == 0 ? 4 : 2, per = 16 / size;
+    constexpr int per = 16 / size;
     uint8_t* p = static_cast<uint8_t*>(a.out) + (r * a.N + n) * size;
     if (vec && n + per <= a.N) {
         *reinterpret_cast<uint4*>(p) = v;
@@ -198,15 +210,24 @@ __device__ __forceinline__ void staging_free() {
     __syncwarp();
 }
 
+// Fills the lane's row of the staged lines.
+__device__ __forceinline__ void refill_row(uint8_t* so, int lines, uint32_t v) {
+    uint8_t* p = so + (threadIdx.x & 31) * 128;
+#pragma unroll 1
+    for (int i = 0; i < lines * 8; ++i)
+        *reinterpret_cast<uint4*>(p + (i >> 3) * 4096 + (i & 7) * 16) = make_uint4(v, v, v, v);
+}
+
 // Sends a warp's staged lines (32 rows x 128 bytes, 16-byte chunks XORed with row % 8, the
 // 128-byte swizzle) to rows r_first + [0, box_rows) and columns n_first on. `whole`: the box may
 // be stored as it is; else only rows below `rows` are, by plain stores.
+template <int size>
 __device__ __forceinline__ void send_lines(const TcArgs& t, const CUtensorMap* tmo, uint8_t* so,
                                            int lines, int64_t r_first, int64_t rows, int64_t n_first,
                                            bool whole) {
     const Fp8Args& a = t.f;
     const int lane = threadIdx.x & 31;
-    const int size = a.out_dtype == 0 ? 4 : 2, per = 128 / size;
+    constexpr int per = 128 / size;
     const int box_rows = min(t.tile_rows, 32);
     if (t.out_tma && whole) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -226,17 +247,19 @@ __device__ __forceinline__ void send_lines(const TcArgs& t, const CUtensorMap* t
         const uint4 u = *reinterpret_cast<const uint4*>(so + line * 4096 + rr * 128 +
                                                         (((lane & 7) ^ (rr & 7)) << 4));
         const int64_t n = n_first + line * per + (lane & 7) * (per / 8);
-        if (rr < box_rows && r_first + rr < rows && n < a.N) store16(a, t.out_tma, r_first + rr, n, u);
+        if (rr < box_rows && r_first + rr < rows && n < a.N) store16<size>(a, t.out_tma, r_first + rr, n, u);
     }
 }
 
-template <int BN, bool SILU, bool SPLIT>
+// Out: the output's type; void selects the SiLU form.
+template <int BN, int TR, typename Out, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
               const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmo) {
-    using C = Cfg<BN>;
+    using C = Cfg<BN, TR>;
+    constexpr bool SILU = std::is_void<Out>::value;
     extern __shared__ uint8_t smem_raw[];
-    Smem<BN>& sm = *reinterpret_cast<Smem<BN>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    Smem<BN, TR>& sm = *reinterpret_cast<Smem<BN, TR>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const Fp8Args& a = t.f;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* bad = &sm.bad;
@@ -372,29 +395,58 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             };
             const int64_t NB = (a.N + kBlk - 1) / kBlk;
             int done = 0;
-            for (Walk w = cur; w.more(); w.next()) {
-                const int e = expert_of(w.rb);
-                const bool present = e >= 0 && e < a.E;
-                const int64_t r0 = (int64_t)w.rb * t.tile_rows, r = r0 + row;
-                const int64_t src = row < t.tile_rows ? source_row(a, r, rows, e) : -1;
+            // The scales of a tile's first block are fetched while the tile before it folds its
+            // last one, its routing entries a whole tile ahead: neither wait is paid per tile.
+            const float *xs = a.xs, *ws0 = a.ws, *ws1 = a.ws;
+            float sx = 0.f, s0 = 0.f, s1 = 0.f;
+            bool present = false, dead = true;  // of tile w, set by enter()
+            int next_e = -1, next_slot = -1;    // of the tile to enter next
+            auto look = [&](const Walk& w) {
+                if (!w.more()) return;
+                const int64_t r = (int64_t)w.rb * t.tile_rows + row;
+                next_e = expert_of(w.rb);
+                next_slot = row >= t.tile_rows || r >= rows ? -1 : a.sorted_ids ? a.sorted_ids[r] : (int)r;
+            };
+            auto enter = [&](const Walk& w) {
+                const int e = next_e;
+                present = e >= 0 && e < a.E;
+                int src = next_slot;
+                if (a.sorted_ids) src = src >= 0 && src < a.num_slots ? src / a.top_k : -1;
+                dead = !present || src < 0;
+                if (!present) return;
                 const int64_t n0 = (int64_t)w.nt * n_step;
+                const int64_t b0 = SILU ? n0 / kBlk : min((n0 + half * C::kCols) / kBlk, NB - 1);
+                xs = a.xs + (int64_t)max(src, 0) * G;
+                ws0 = a.ws + (e * NB + b0) * G;
+                ws1 = SILU ? ws0 + (a.N / 2 / kBlk) * G : ws0;
+                if (g_lo < g_hi) {
+                    sx = __ldg(xs + g_lo);
+                    s0 = __ldg(ws0 + g_lo);
+                    if (SILU) s1 = __ldg(ws1 + g_lo);
+                }
+            };
+            Walk w = cur;
+            look(w);
+            if (w.more()) enter(w);
+            while (w.more()) {
+                const int64_t r0 = (int64_t)w.rb * t.tile_rows, r = r0 + row;
+                const int64_t n0 = (int64_t)w.nt * n_step;
+                const bool is_dead = dead, is_present = present && g_lo < g_hi;
+                w.next();
+                if (!SPLIT) look(w);
                 float tot[C::kCols];
 #pragma unroll
                 for (int j = 0; j < C::kCols; ++j) tot[j] = 0.f;
-                if (present) {
-                    const float* xs = a.xs + max(src, (int64_t)0) * G;
-                    const int64_t b0 = SILU ? n0 / kBlk : min((n0 + half * C::kCols) / kBlk, NB - 1);
-                    const float* ws0 = a.ws + (e * NB + b0) * G;
-                    const float* ws1 = SILU ? ws0 + (a.N / 2 / kBlk) * G : ws0;
-                    float sx = g_lo < g_hi ? __ldg(xs + g_lo) : 0.f;
-                    float s0 = g_lo < g_hi ? __ldg(ws0 + g_lo) : 0.f;
-                    float s1 = SILU && g_lo < g_hi ? __ldg(ws1 + g_lo) : 0.f;
+                if (!is_present && !SPLIT && w.more()) enter(w);
+                if (is_present) {
                     for (int g = g_lo; g < g_hi; ++g) {
                         const float f0 = sx * s0, f1 = SILU ? sx * s1 : f0;
                         if (g + 1 < g_hi) {  // the next block's scales, behind this block's fold
                             sx = __ldg(xs + g + 1);
                             s0 = __ldg(ws0 + g + 1);
                             if (SILU) s1 = __ldg(ws1 + g + 1);
+                        } else if (!SPLIT && w.more()) {
+                            enter(w);
                         }
                         mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::);
@@ -404,7 +456,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         tmem_wait16(v[0]);
 #pragma unroll
                         for (int j = 0; j < C::kCols; j += 16) {
-                            uint32_t(&cur)[16] = v[(j / 16) & 1];
+                            uint32_t(&now)[16] = v[(j / 16) & 1];
                             uint32_t(&nxt)[16] = v[(j / 16 + 1) & 1];
                             if (j + 16 < C::kCols) tmem_ld16_nowait(base + col(j + 16), nxt);
                             const float f = j < C::kCols / 2 ? f0 : f1;
@@ -412,7 +464,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) {
                                 const float2 p = ffma2(
-                                    make_float2(__uint_as_float(cur[i]), __uint_as_float(cur[i + 1])),
+                                    make_float2(__uint_as_float(now[i]), __uint_as_float(now[i + 1])),
                                     f2, make_float2(tot[j + i], tot[j + i + 1]));
                                 tot[j + i] = p.x;
                                 tot[j + i + 1] = p.y;
@@ -425,10 +477,10 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         tb.next();
                     }
                 }
-                // rows of zeros stay zero whatever the lane's accumulator held
-                const float poison = *bad ? __int_as_float(0x7fffffff) : 0.f;
-#pragma unroll
-                for (int j = 0; j < C::kCols; ++j) tot[j] = src < 0 ? poison : tot[j] + poison;
+                // rows of zeros are zero whatever the lane's accumulator held: such a lane writes
+                // `fill` over its staged row (a wait that gave up makes every row one, of NaN)
+                const bool refill = is_dead || *bad;
+                const float fill = *bad ? __int_as_float(0x7fffffff) : 0.f;
                 if (SPLIT) {
                     // park the partial tile; the ring is idle once the last accumulator was read
                     if (row < t.tile_rows) {
@@ -437,14 +489,19 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         for (int j = 0; j < C::kCols; j += 4)
                             *reinterpret_cast<float4*>(part + col(j)) =
                                 make_float4(tot[j], tot[j + 1], tot[j + 2], tot[j + 3]);
+                        if (refill)
+#pragma unroll 1
+                            for (int j = 0; j < C::kCols; ++j)
+                                part[SILU ? (j & 63) + (j >> 6) * 128 + half * 64 : half * C::kCols + j] = fill;
                     }
-                } else if (SILU) {
+                } else if constexpr (SILU) {
                     float m = 0.f;
 #pragma unroll
                     for (int j = 0; j < 64; ++j) {
                         tot[j] = silu_mul(tot[j], tot[(j + 64) % C::kCols]);
                         m = fmaxf(m, fabsf(tot[j]));
                     }
+                    if (refill) m = fill;
                     // the row's other 64 outputs are with the warp of the other half
                     float* amax = reinterpret_cast<float*>(sm.stage_out) + (done & 1) * 256;
                     amax[half * 128 + row] = m;
@@ -465,11 +522,16 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                                        (uint32_t)quant_pair(tot[j + 4 * i + 2], tot[j + 4 * i + 3], s, rcp) << 16;
                             qp[j / 16] = make_uint4(u[0], u[1], u[2], u[3]);
                         }
+                        if (refill) {
+                            const uint32_t z = fill == 0.f ? 0u : 0x7f7f7f7fu;
+#pragma unroll 1
+                            for (int j = 0; j < 4; ++j) qp[j] = make_uint4(z, z, z, z);
+                        }
                     }
                 } else {
-                    uint8_t* so = sm.stage_out[fw][0];
+                    uint8_t* so = sm.stage_out[TR == 32 ? half : fw][0];
                     const bool whole = !a.ntp || r0 + q * 32 + min(t.tile_rows, 32) <= rows;
-                    if (a.out_dtype == 0) {
+                    if constexpr (sizeof(Out) == 4) {
 #pragma unroll
                         for (int c0 = 0; c0 < C::kCols; c0 += C::kCols / 2) {  // 32 columns a line
                             staging_free();
@@ -479,21 +541,23 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                                                            (((c / 4 % 8) ^ (lane & 7)) << 4)) =
                                     make_float4(tot[c0 + c], tot[c0 + c + 1], tot[c0 + c + 2],
                                                 tot[c0 + c + 3]);
-                            send_lines(t, &tmo, so, C::kLines, r0 + q * 32, rows, n0 + col(c0), whole);
+                            if (refill) refill_row(so, C::kLines, __float_as_uint(fill));
+                            send_lines<sizeof(Out)>(t, &tmo, so, C::kLines, r0 + q * 32, rows, n0 + col(c0), whole);
                         }
                     } else {
                         staging_free();
 #pragma unroll
                         for (int c = 0; c < C::kCols; c += 8) {  // 64 columns a line
                             uint4 u;
-                            u.x = pack2(a.out_dtype, tot[c], tot[c + 1]);
-                            u.y = pack2(a.out_dtype, tot[c + 2], tot[c + 3]);
-                            u.z = pack2(a.out_dtype, tot[c + 4], tot[c + 5]);
-                            u.w = pack2(a.out_dtype, tot[c + 6], tot[c + 7]);
+                            u.x = pack2<Out>(tot[c], tot[c + 1]);
+                            u.y = pack2<Out>(tot[c + 2], tot[c + 3]);
+                            u.z = pack2<Out>(tot[c + 4], tot[c + 5]);
+                            u.w = pack2<Out>(tot[c + 6], tot[c + 7]);
                             *reinterpret_cast<uint4*>(so + (c / 64) * 4096 + lane * 128 +
                                                       (((c / 8 % 8) ^ (lane & 7)) << 4)) = u;
                         }
-                        send_lines(t, &tmo, so, C::kLines, r0 + q * 32, rows, n0 + col(0), whole);
+                        if (refill) refill_row(so, C::kLines, pack2<Out>(fill, fill));
+                        send_lines<sizeof(Out)>(t, &tmo, so, C::kLines, r0 + q * 32, rows, n0 + col(0), whole);
                     }
                 }
                 ++done;
@@ -531,7 +595,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             sum[c].w += v[k].w;
                         }
                 }
-                if (SILU) {
+                if constexpr (SILU) {
                     const float4 g4 = sum[0], u4 = sum[BN / 128 - 1];
                     const float h[4] = {silu_mul(g4.x, u4.x), silu_mul(g4.y, u4.y),
                                         silu_mul(g4.z, u4.z), silu_mul(g4.w, u4.w)};
@@ -550,7 +614,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     for (int c = 0; c < BN / 128; ++c) {
                         const int64_t n = n0 + c * 128 + 4 * lane;
                         const float o[4] = {sum[c].x, sum[c].y, sum[c].z, sum[c].w};
-                        if (a.out_dtype == 0) {
+                        if constexpr (sizeof(Out) == 4) {
                             float* p = static_cast<float*>(a.out) + r * a.N + n;
                             if (vec && n + 4 <= a.N) *reinterpret_cast<float4*>(p) = sum[c];
                             else
@@ -559,8 +623,8 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                                     if (n + i < a.N) p[i] = o[i];
                         } else {
                             uint16_t* p = static_cast<uint16_t*>(a.out) + r * a.N + n;
-                            const uint32_t lo = pack2(a.out_dtype, o[0], o[1]);
-                            const uint32_t hi = pack2(a.out_dtype, o[2], o[3]);
+                            const uint32_t lo = pack2<Out>(o[0], o[1]);
+                            const uint32_t hi = pack2<Out>(o[2], o[3]);
                             if (vec && n + 4 <= a.N) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
                             else
 #pragma unroll
@@ -600,8 +664,9 @@ int sm_count() {
     return n > 0 ? n : 148;
 }
 
-template <int BN, bool SILU, bool SPLIT>
+template <int BN, int TR, typename Out, bool SPLIT>
 int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
+    constexpr bool SILU = std::is_void<Out>::value;
     const Fp8Args& a = t.f;
     CUtensorMap tmx, tmw, tmo{};
     const int64_t pitch = a.N * (a.out_dtype == 0 ? 4 : 2);
@@ -615,8 +680,8 @@ int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
         !make_tma_map_u8(&tmw, a.w, (uint64_t)(a.E * a.N), (uint64_t)a.K, 128, 128,
                          CU_TENSOR_MAP_SWIZZLE_128B))
         return set_error("fp8_block: tensor map encoding failed");
-    auto kern = fp8_tc_kernel<BN, SILU, SPLIT>;
-    const int smem = (int)sizeof(Smem<BN>) + 1024;
+    auto kern = fp8_tc_kernel<BN, TR, Out, SPLIT>;
+    const int smem = (int)sizeof(Smem<BN, TR>) + 1024;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg{};
@@ -632,6 +697,25 @@ int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
     e = cudaLaunchKernelEx(&cfg, kern, t, tmx, tmw, tmo);
     if (e != cudaSuccess) return (int)e;
     return launch_status();
+}
+
+template <int TR, typename Out>
+int launch_out(const TcArgs& t, bool bn256, int64_t tiles, cudaStream_t st) {
+    if (bn256) return launch_t<256, TR, Out, false>(t, tiles, st);
+    return t.split > 1 ? launch_t<128, TR, Out, true>(t, tiles, st)
+                       : launch_t<128, TR, Out, false>(t, tiles, st);
+}
+
+template <int TR>
+int launch_tr(const TcArgs& t, bool bn256, int64_t tiles, cudaStream_t st) {
+    if (t.f.silu)
+        return t.split > 1 ? launch_t<256, TR, void, true>(t, tiles, st)
+                           : launch_t<256, TR, void, false>(t, tiles, st);
+    switch (t.f.out_dtype) {
+        case 0: return launch_out<TR, float>(t, bn256, tiles, st);
+        case 1: return launch_out<TR, __half>(t, bn256, tiles, st);
+        default: return launch_out<TR, __nv_bfloat16>(t, bn256, tiles, st);
+    }
 }
 
 }  // namespace
@@ -660,11 +744,7 @@ int launch_fp8_tc(const Fp8Args& a, cudaStream_t st) {
     t.n_tiles = (int)(tiles / blocks);
     t.split = 1;
     while (t.split < kMaxSplit && tiles * t.split * 2 <= sms && a.G >= t.split * 4) t.split *= 2;
-    const bool split = t.split > 1;
-    if (a.silu)
-        return split ? launch_t<256, true, true>(t, tiles, st) : launch_t<256, true, false>(t, tiles, st);
-    if (bn256) return launch_t<256, false, false>(t, tiles, st);
-    return split ? launch_t<128, false, true>(t, tiles, st) : launch_t<128, false, false>(t, tiles, st);
+    return t.tile_rows <= 32 ? launch_tr<32>(t, bn256, tiles, st) : launch_tr<128>(t, bn256, tiles, st);
 }
 
 }  // namespace w4a8
