@@ -9,12 +9,13 @@
 // has to be read, still pass at the MMA's full N rate, and rows that do not exist are not loaded,
 // folded or stored.
 //
-// One persistent CTA per SM, 10 warps:
+// One persistent CTA per SM, 12 warps:
 //   warp 0     TMA producer: per stage one 128-byte column slab of the tile's x rows (a 2D box, or
 //              tile::gather4 through the routing, one 4-row gather per lane) and BN weight rows,
 //              in the 128-byte swizzle that the MMA's K-major descriptors read.
 //   warp 1     owns tensor memory; one thread issues 4 x tcgen05.mma.kind::f8f6f4 (K = 32) per
 //              block into a ring of fp32 accumulators (512 / BN of them).
+//   warps 10, 11  copy the x rows of tall routed tiles (64 or 128 rows) with cp.async instead.
 //   warps 2-9  fold: lane quarter warp % 4, one half of the columns each; then the epilogue.
 //
 // When there are fewer tiles than SMs, a cluster of S CTAs shares a tile: each takes a slice of
@@ -42,7 +43,8 @@ namespace w4a8 {
 namespace {
 
 constexpr int kBlk = 128;
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
+constexpr int kGatherWarps = 2;  // warps 10 and 11
 constexpr int kFoldWarps = 8;
 constexpr int kMaxSplit = 8;
 
@@ -169,6 +171,14 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
     return __fdividef(g, 1.f + __expf(-g)) * u;
 }
 
+// Four e4m3 bytes of v / scale, rcp = 1 / scale. The values carry more than the 2^-23 by which the
+// product may miss the quotient; the exact quotient's slow path, 32 times inlined, cost 5x the
+// whole epilogue in instruction fetches.
+__device__ __forceinline__ uint32_t quant4(float v0, float v1, float v2, float v3, float rcp) {
+    return (uint32_t)f32x2_to_e4m3x2(v0 * rcp, v1 * rcp) |
+           (uint32_t)f32x2_to_e4m3x2(v2 * rcp, v3 * rcp) << 16;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
@@ -273,13 +283,17 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     const int g_lo = (int)((int64_t)G * rank / S), g_hi = (int)((int64_t)G * (rank + 1) / S);
     const int live_warps = 2 * ((t.tile_rows + 31) / 32);  // fold warps whose lanes hold rows
     const int n_step = SILU ? 128 : BN;                    // outputs per tile
+    // rows in routing order: short tiles by gather4 (72 cycles of issue per 4 rows), tall ones by
+    // the gather warps' copies (128 rows of gather4 took 2300 cycles a stage, the MMAs 600)
+    const bool copy_rows = TR == 128 && a.sorted_ids != nullptr;
+    const bool tma_gather = TR == 32 && a.sorted_ids != nullptr;
     const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
     auto expert_of = [&](int rb) { return a.expert_ids ? a.expert_ids[rb / per_expert] : 0; };
 
     if (tid == 0) {
         sm.bad = 0;
         for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.full[s], copy_rows ? 1 + kGatherWarps : 1);
             mbar_init(&sm.empty[s], 1);
         }
         for (int s = 0; s < C::kAcc; ++s) {
@@ -308,7 +322,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     do {
     if (warp == 0) {
         // ---------------- TMA producer ----------------
-        const uint32_t stage_bytes = (uint32_t)t.tile_rows * 128 + C::kBBytes;
+        const uint32_t stage_bytes = (copy_rows ? 0u : (uint32_t)t.tile_rows * 128) + C::kBBytes;
         for (Walk w = cur; w.more(); w.next()) {
             const int e = expert_of(w.rb);
             if (e < 0 || e >= a.E) {
@@ -317,7 +331,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             }
             const int r0 = w.rb * t.tile_rows;
             int src[4] = {0, 0, 0, 0};  // gathered rows 4 * lane + i; padding rows read row 0
-            if (a.sorted_ids && 4 * lane < t.tile_rows)
+            if (tma_gather && 4 * lane < t.tile_rows)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     src[i] = (int)max((int64_t)0, source_row(a, r0 + 4 * lane + i, rows, e));
@@ -336,7 +350,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     if (!a.sorted_ids) tma_load_2d(xa, &tmx, g * 128, r0, fb);
                 }
                 __syncwarp();
-                if (a.sorted_ids && 4 * lane < t.tile_rows)
+                if (tma_gather && 4 * lane < t.tile_rows)
                     tma_gather4(xa + lane * 512, &tmx, g * 128, src, fb);
                 st.next();
                 ++issued;
@@ -381,6 +395,74 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 }
                 if (SPLIT) break;
             }
+        }
+        __syncwarp();
+    } else if (warp >= 2 + kFoldWarps) {
+        // ---------------- gather warps: x rows in routing order, tall tiles ----------------
+        // Lane l copies 16-byte chunk l % 8 of rows (l / 8) + 4 (warp index) + 8 i; a stage is
+        // announced when the next one has been requested, so that two are in flight.
+        if (copy_rows) {
+            constexpr int kRowsPer = TR / (4 * kGatherWarps);
+            const int chunk = lane & 7, row0 = (warp - 2 - kFoldWarps) * 4 + (lane >> 3);
+            int pending = -1;  // stage requested but not announced
+            auto announce = [&](int stage) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.full[stage]);
+            };
+            int slot[kRowsPer], e = -1;  // of the tile to enter next, fetched a tile ahead
+            auto look = [&](const Walk& w) {
+                if (!w.more()) return;
+                e = expert_of(w.rb);
+#pragma unroll
+                for (int i = 0; i < kRowsPer; ++i) {
+                    const int tr = row0 + i * 4 * kGatherWarps;
+                    const int64_t r = (int64_t)w.rb * t.tile_rows + tr;
+                    slot[i] = tr < t.tile_rows && r < rows ? a.sorted_ids[r] : -1;
+                }
+            };
+            Walk w = cur;
+            look(w);
+            while (w.more()) {
+                const bool present = e >= 0 && e < a.E;
+                int src[kRowsPer];
+#pragma unroll
+                for (int i = 0; i < kRowsPer; ++i)
+                    src[i] = slot[i] >= 0 && slot[i] < a.num_slots ? slot[i] / a.top_k : -1;
+                w.next();
+                if (!SPLIT) look(w);
+                if (!present) {
+                    if (SPLIT) break;
+                    continue;
+                }
+                for (int g = g_lo; g < g_hi; ++g) {
+                    mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
+                    const int64_t k = (int64_t)g * kBlk + chunk * 16;
+                    const uint32_t xa = smem_u32(sm.ring[st.idx]);
+#pragma unroll
+                    for (int i = 0; i < kRowsPer; ++i) {
+                        const int tr = row0 + i * 4 * kGatherWarps;
+                        if (tr >= t.tile_rows) break;
+                        // absent rows and columns past K are written as zeros (source size 0)
+                        const bool ok = src[i] >= 0 && k < a.K;
+                        const uint8_t* p = a.x + (ok ? (int64_t)src[i] * a.K + k : 0);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         xa + tr * 128 + ((chunk ^ (tr & 7)) << 4)),
+                                     "l"(p), "r"(ok ? 16 : 0)
+                                     : "memory");
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (pending >= 0) {
+                        asm volatile("cp.async.wait_group 1;" ::: "memory");
+                        announce(pending);
+                    }
+                    pending = (int)st.idx;
+                    st.next();
+                }
+                if (SPLIT) break;
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (pending >= 0) announce(pending);
         }
         __syncwarp();
     } else {
@@ -518,8 +600,8 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             uint32_t u[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                u[i] = (uint32_t)quant_pair(tot[j + 4 * i], tot[j + 4 * i + 1], s, rcp) |
-                                       (uint32_t)quant_pair(tot[j + 4 * i + 2], tot[j + 4 * i + 3], s, rcp) << 16;
+                                u[i] = quant4(tot[j + 4 * i], tot[j + 4 * i + 1], tot[j + 4 * i + 2],
+                                              tot[j + 4 * i + 3], rcp);
                             qp[j / 16] = make_uint4(u[0], u[1], u[2], u[3]);
                         }
                         if (refill) {
@@ -571,7 +653,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     if (SPLIT) {
         // CTA `rank` finishes rows rank, rank + S, ... of the cluster's tile
         cluster_sync();
-        if (warp >= 2 && cur.more()) {
+        if (warp >= 2 && warp < 2 + kFoldWarps && cur.more()) {
             const int64_t r0 = (int64_t)cur.rb * t.tile_rows, n0 = (int64_t)cur.nt * n_step;
             const bool vec = t.out_tma;
             const float* part = reinterpret_cast<const float*>(sm.ring);
@@ -607,8 +689,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     const int64_t inter = a.N / 2;
                     if (lane == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
                     *reinterpret_cast<uint32_t*>(a.q + r * inter + n0 + 4 * lane) =
-                        (uint32_t)quant_pair(h[0], h[1], s, rcp) |
-                        (uint32_t)quant_pair(h[2], h[3], s, rcp) << 16;
+                        quant4(h[0], h[1], h[2], h[3], rcp);
                 } else {
 #pragma unroll
                     for (int c = 0; c < BN / 128; ++c) {
