@@ -52,6 +52,171 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Eight consecutive values, packed as they lie in memory.
+template <typename T>
+struct Vec8 {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    }
+    // a buffer that this kernel also writes (the residual, updated in place): no read-only path
+    __device__ __forceinline__ void load_rw(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = *(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(w)[i]); }
+    __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(w)[i] = from_f32<T>(v); }
+};
+
+// e4m3 bytes of v / s, IEEE quotients. With r the correctly rounded reciprocal of s and y = v r,
+// the quotient's correctly rounded value is y + (v - y s) r, both steps fused multiply-adds
+// (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).
+// An infinite s has r = 0; its residual is taken with s = 0, which leaves y, as the divide would.
+// Where the residual underflows, the quotient is far below e4m3's smallest value.
+__device__ __forceinline__ float quotient(float v, float s, float r) {
+    const float y = __fmul_rn(v, r);
+    return copysignf(__fmaf_rn(__fmaf_rn(-y, s, v), r, y), v);  // -0 has no residual to keep its sign
+}
+
+__device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale) {
+    const float r = __frcp_rn(scale), s = isinf(scale) ? 0.f : scale;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = quotient(v[i], s, r);
+    return make_uint2((uint32_t)f32x2_to_e4m3x2(y[0], y[1]) | (uint32_t)f32x2_to_e4m3x2(y[2], y[3]) << 16,
+                      (uint32_t)f32x2_to_e4m3x2(y[4], y[5]) | (uint32_t)f32x2_to_e4m3x2(y[6], y[7]) << 16);
+}
+
+// 16 lanes quantise one block, 8 values each (zeros past the row's end).
+__device__ __forceinline__ uint2 quant_block_half(const float (&v)[8], float& s) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
+    amax = lanes_max<16>(amax);
+    s = __fdiv_rn(fmaxf(amax, kAmaxFloor), kE4m3Max);
+    return quant8(v, s);
+}
+
+// K % 8 == 0 and aligned rows: 16 lanes per block, kPerHalf blocks each, all requested first.
+constexpr int kPerHalf = 4;
+template <typename T>
+__global__ void __launch_bounds__(256)
+act_quant_block_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                           float* __restrict__ scales, int64_t blocks, uint32_t K, uint32_t G) {
+    const int sub = threadIdx.x & 15;
+    const int64_t b0 = (int64_t)blockIdx.x * (16 * kPerHalf) + (threadIdx.x >> 4);
+    Vec8<T> x8[kPerHalf];
+    int64_t at[kPerHalf];
+#pragma unroll
+    for (int i = 0; i < kPerHalf; ++i) {
+        const int64_t b = b0 + i * 16;
+        at[i] = -1;
+        x8[i].zero();
+        if (b < blocks) {
+            const int64_t r = blocks <= INT32_MAX ? (int64_t)((uint32_t)b / G) : b / G;
+            const uint32_t k = (uint32_t)(b - r * G) * kBlk + sub * 8;
+            if (k < K) {
+                at[i] = r * K + k;
+                x8[i].load(x + at[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPerHalf; ++i) {
+        const int64_t b = b0 + i * 16;
+        float v[8], s;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x8[i].get(j);
+        const uint2 u = quant_block_half(v, s);
+        if (sub == 0 && b < blocks) scales[b] = s;
+        if (at[i] >= 0) *reinterpret_cast<uint2*>(q + at[i]) = u;
+    }
+}
+
+// The norm with the row in registers: kThreads threads per row, V vectors of 8 each (vector j of
+// thread t is j * kThreads + t, so 16 neighbours hold one block). A CTA walks rows with the
+// weights kept; rows of H % 8 == 0 elements, H <= 8 V kThreads, aligned.
+template <typename T, typename W, int kThreads, int V>
+__global__ void __launch_bounds__(kThreads)
+rms_norm_quant_vec_kernel(const T* __restrict__ x, const T* residual, const W* __restrict__ weight,
+                          float eps, int64_t M, uint32_t H, uint32_t G, uint8_t* __restrict__ q,
+                          float* __restrict__ scales, T* residual_out, T* __restrict__ normed) {
+    __shared__ float part[2][kThreads / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t vecs = H / 8;
+    Vec8<W> w8[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        w8[j].zero();
+        if (j * kThreads + tid < vecs) w8[j].load(weight + (j * kThreads + tid) * 8);
+    }
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < M; r += gridDim.x, turn ^= 1) {
+        const int64_t base = r * H;
+        Vec8<T> x8[V], r8[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t n = j * kThreads + tid;
+            x8[j].zero();
+            r8[j].zero();
+            if (n < vecs) {
+                x8[j].load(x + base + n * 8);
+                if (residual) r8[j].load_rw(residual + base + n * 8);
+            }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (residual) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x8[j].set(i, x8[j].get(i) + r8[j].get(i));
+                const uint32_t n = j * kThreads + tid;
+                if (n < vecs) x8[j].store(residual_out + base + n * 8);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float h = x8[j].get(i);
+                ss += h * h;
+            }
+        }
+        ss = warp_sum(ss);
+        if (lane == 0) part[turn][warp] = ss;
+        __syncthreads();  // the next row writes the other half of `part`
+        float tot = 0.f;
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i) tot += part[turn][i];
+        const float rstd = rsqrtf(tot / (float)H + eps);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t n = j * kThreads + tid;
+            float v[8], s;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = n < vecs ? x8[j].get(i) * rstd * w8[j].get(i) : 0.f;
+            const uint2 u = quant_block_half(v, s);
+            if (n < vecs) {
+                if ((tid & 15) == 0) scales[r * G + n / 16] = s;
+                *reinterpret_cast<uint2*>(q + base + n * 8) = u;
+                if (normed) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x8[j].set(i, v[i]);
+                    x8[j].store(normed + base + n * 8);
+                }
+            }
+        }
+    }
+}
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
 // One warp quantises one block of up to 128 values: v[j] is column lane + 32 j of the block.
 __device__ __forceinline__ void quant_block_warp(const float (&v)[4], int cols, uint8_t* q,
                                                  float* scale) {
@@ -92,10 +257,10 @@ act_quant_block_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
 // more (from L2) for the output.
 template <typename T, typename W>
 __global__ void __launch_bounds__(256)
-rms_norm_quant_kernel(const T* __restrict__ x, const T* __restrict__ residual,
+rms_norm_quant_kernel(const T* __restrict__ x, const T* residual,
                       const W* __restrict__ weight, float eps, int64_t H, int64_t G,
                       uint8_t* __restrict__ q, float* __restrict__ scales,
-                      T* __restrict__ residual_out, T* __restrict__ normed) {
+                      T* residual_out, T* __restrict__ normed) {
     __shared__ float part[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t base = (int64_t)blockIdx.x * H;
@@ -138,6 +303,14 @@ rms_norm_quant_kernel(const T* __restrict__ x, const T* __restrict__ residual,
 template <typename T>
 int launch_quant(const void* x, int64_t M, int64_t K, uint8_t* q, float* scales, cudaStream_t st) {
     const int64_t G = (K + kBlk - 1) / kBlk, blocks = M * G;
+    if (K % 8 == 0 && aligned(x, 16) && aligned(q, 8)) {
+        const int64_t ctas = (blocks + 16 * kPerHalf - 1) / (16 * kPerHalf);
+        if (ctas <= INT32_MAX) {
+            act_quant_block_vec_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(
+                static_cast<const T*>(x), q, scales, blocks, (uint32_t)K, (uint32_t)G);
+            return launch_status();
+        }
+    }
     const int64_t want = (blocks + 7) / 8;
     const unsigned grid = (unsigned)(want < 148 * 64 ? want : 148 * 64);
     act_quant_block_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(x), q, scales, blocks, K, G);
@@ -153,8 +326,31 @@ struct NormArgs {
     void *residual_out, *normed;
 };
 
+template <typename T, typename W, int kThreads, int V>
+int launch_norm_vec(const NormArgs& a, cudaStream_t st) {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int64_t most = (int64_t)sms * (2048 / kThreads);
+    rms_norm_quant_vec_kernel<T, W, kThreads, V><<<(unsigned)(a.M < most ? a.M : most), kThreads, 0, st>>>(
+        static_cast<const T*>(a.x), static_cast<const T*>(a.residual),
+        static_cast<const W*>(a.weight), a.eps, a.M, (uint32_t)a.H,
+        (uint32_t)((a.H + kBlk - 1) / kBlk), a.q, a.scales, static_cast<T*>(a.residual_out),
+        static_cast<T*>(a.normed));
+    return launch_status();
+}
+
 template <typename T, typename W>
 int launch_norm(const NormArgs& a, cudaStream_t st) {
+    if (a.H % 8 == 0 && a.H <= 16384 && aligned(a.x, 16) && aligned(a.residual, 16) &&
+        aligned(a.weight, 16) && aligned(a.q, 8) && aligned(a.residual_out, 16) &&
+        aligned(a.normed, 16)) {
+        if (a.H <= 1024) return launch_norm_vec<T, W, 128, 1>(a, st);
+        if (a.H <= 2048) return launch_norm_vec<T, W, 128, 2>(a, st);
+        if (a.H <= 4096) return launch_norm_vec<T, W, 256, 2>(a, st);
+        if (a.H <= 8192) return launch_norm_vec<T, W, 256, 4>(a, st);
+        return launch_norm_vec<T, W, 512, 4>(a, st);
+    }
     rms_norm_quant_kernel<T, W><<<(unsigned)a.M, 256, 0, st>>>(
         static_cast<const T*>(a.x), static_cast<const T*>(a.residual),
         static_cast<const W*>(a.weight), a.eps, a.H, (a.H + kBlk - 1) / kBlk, a.q, a.scales,

@@ -8,6 +8,7 @@
 // non-zero status. There is no CPU kernel: a CPU tensor fails the is_cuda check.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -505,6 +506,12 @@ bool is_e4m3(const at::Tensor& t) {
     return t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kByte;
 }
 
+// An output on x's device, straight from the CUDA allocator: at::empty's trip through the
+// dispatcher costs about 1 us each, which is what these calls are made of at decode sizes.
+at::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& x) {
+    return at::detail::empty_cuda(sizes, dtype, x.device(), c10::nullopt);
+}
+
 std::vector<at::Tensor> act_quant_fp8_block_forward(const at::Tensor& x) {
     TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(),
                 "x must be a contiguous (M, K) CUDA tensor");
@@ -512,8 +519,8 @@ std::vector<at::Tensor> act_quant_fp8_block_forward(const at::Tensor& x) {
     const int64_t M = x.size(0), K = x.size(1);
     TORCH_CHECK(K > 0, "x must have at least one column");
     const c10::cuda::CUDAGuard guard(x.device());
-    auto q = at::empty({M, K}, x.options().dtype(at::kFloat8_e4m3fn));
-    auto s = at::empty({M, scale_blocks(K)}, x.options().dtype(at::kFloat));
+    auto q = new_cuda({M, K}, at::kFloat8_e4m3fn, x);
+    auto s = new_cuda({M, scale_blocks(K)}, at::kFloat, x);
     check_status(w4a8_act_quant_fp8_block(x.data_ptr(), dt, M, K, static_cast<uint8_t*>(q.data_ptr()),
                                           s.data_ptr<float>(), cur_stream()),
                  "act_quant_fp8_block");
@@ -540,10 +547,10 @@ std::vector<at::Tensor> rms_norm_quant_fp8_forward(const at::Tensor& x, const at
                         residual->scalar_type() == x.scalar_type() && residual->is_contiguous(),
                     "residual must be contiguous with x's shape, type and device");
     const c10::cuda::CUDAGuard guard(x.device());
-    auto q = at::empty({M, H}, x.options().dtype(at::kFloat8_e4m3fn));
-    auto s = at::empty({M, scale_blocks(H)}, x.options().dtype(at::kFloat));
-    auto res = residual ? at::empty_like(x) : at::empty({0}, x.options());
-    auto nrm = with_normed ? at::empty_like(x) : at::empty({0}, x.options());
+    auto q = new_cuda({M, H}, at::kFloat8_e4m3fn, x);
+    auto s = new_cuda({M, scale_blocks(H)}, at::kFloat, x);
+    auto res = new_cuda({residual ? M : 0, H}, x.scalar_type(), x);
+    auto nrm = new_cuda({with_normed ? M : 0, H}, x.scalar_type(), x);
     // an empty batch has no storage to point at; there is nothing to launch either
     if (M > 0)
         check_status(w4a8_rms_norm_quant_fp8(
@@ -581,7 +588,7 @@ at::Tensor fp8_block_gemm_forward(const at::Tensor& x, const at::Tensor& x_scale
                 "w_scales must be contiguous fp32 (ceil(N/128), ceil(K/128)) on x's device");
     const int32_t dt = dtype_code(out_dtype, "out_dtype");
     const c10::cuda::CUDAGuard guard(x.device());
-    auto out = at::empty({M, N}, x.options().dtype(out_dtype));
+    auto out = new_cuda({M, N}, out_dtype, x);
     check_status(w4a8_fp8_block_gemm(static_cast<const uint8_t*>(x.data_ptr()),
                                      x_scales.data_ptr<float>(),
                                      static_cast<const uint8_t*>(w.data_ptr()),
@@ -632,7 +639,7 @@ at::Tensor fp8_block_moe_gemm_forward(const at::Tensor& x, const at::Tensor& x_s
     const int64_t P = sorted_token_ids ? sorted_token_ids->size(0) : x.size(0);
     const int32_t dt = dtype_code(out_dtype, "out_dtype");
     const c10::cuda::CUDAGuard guard(x.device());
-    auto out = at::empty({P, w.size(1)}, x.options().dtype(out_dtype));
+    auto out = new_cuda({P, w.size(1)}, out_dtype, x);
     check_status(w4a8_fp8_block_moe_gemm(
                      static_cast<const uint8_t*>(x.data_ptr()), x_scales.data_ptr<float>(),
                      static_cast<const uint8_t*>(w.data_ptr()), w_scales.data_ptr<float>(),
@@ -653,8 +660,8 @@ std::vector<at::Tensor> fp8_block_moe_gemm1_silu_forward(
     const int64_t P = sorted_token_ids ? sorted_token_ids->size(0) : x.size(0);
     const int64_t inter = w.size(1) / 2;
     const c10::cuda::CUDAGuard guard(x.device());
-    auto q = at::empty({P, inter}, x.options().dtype(at::kFloat8_e4m3fn));
-    auto s = at::empty({P, inter / kScaleBlock}, x.options().dtype(at::kFloat));
+    auto q = new_cuda({P, inter}, at::kFloat8_e4m3fn, x);
+    auto s = new_cuda({P, inter / kScaleBlock}, at::kFloat, x);
     check_status(w4a8_fp8_block_moe_gemm1_silu(
                      static_cast<const uint8_t*>(x.data_ptr()), x_scales.data_ptr<float>(),
                      static_cast<const uint8_t*>(w.data_ptr()), w_scales.data_ptr<float>(),

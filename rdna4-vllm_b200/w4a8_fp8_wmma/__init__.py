@@ -179,11 +179,18 @@ def route_topk(logits: torch.Tensor, top_k: int, renormalize: bool = True):
 # e4m3 values (float8_e4m3fn, or their uint8 bytes) with one fp32 scale per 128 columns of an
 # activation row and per 128 x 128 block of a weight; the last block of a side may be short.
 
+# the overloads themselves: looking them up at each call costs as much as a decode-size kernel
+_act_quant_fp8_block_op = torch.ops.w4a8_b200.act_quant_fp8_block.default
+_rms_norm_quant_fp8_op = torch.ops.w4a8_b200.rms_norm_quant_fp8.default
+_fp8_block_gemm_op = torch.ops.w4a8_b200.fp8_block_gemm.default
+_fp8_block_moe_gemm_op = torch.ops.w4a8_b200.fp8_block_moe_gemm.default
+_fp8_block_moe_gemm1_silu_op = torch.ops.w4a8_b200.fp8_block_moe_gemm1_silu.default
+
+
 def act_quant_fp8_block(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(M, K) fp16/bf16/fp32 -> (q (M, K) float8_e4m3fn, scales (M, ceil(K/128)) fp32): the rule
     of act_quant_fp8 applied to each 128 columns of a row."""
-    q, s = torch.ops.w4a8_b200.act_quant_fp8_block(x.contiguous())
-    return q, s
+    return tuple(_act_quant_fp8_block_op(x.contiguous()))
 
 
 def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -195,7 +202,7 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     residual or None, y in x's type if with_normed else None). x and residual fp16, bf16 or
     fp32; weight in x's type or fp32.
     """
-    q, s, res, normed = torch.ops.w4a8_b200.rms_norm_quant_fp8(
+    q, s, res, normed = _rms_norm_quant_fp8_op(
         x.contiguous(), weight.contiguous(), float(eps),
         residual.contiguous() if residual is not None else None, bool(with_normed))
     return q, s, (res if residual is not None else None), (normed if with_normed else None)
@@ -209,7 +216,7 @@ def fp8_block_gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor,
     and rounded once. K a multiple of 16 takes the tensor cores; any other K is served by a
     plain kernel.
     """
-    return torch.ops.w4a8_b200.fp8_block_gemm(x, x_scales, w, w_scales, out_dtype)
+    return _fp8_block_gemm_op(x, x_scales, w, w_scales, out_dtype)
 
 
 def fp8_block_moe_gemm(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
@@ -222,7 +229,7 @@ def fp8_block_moe_gemm(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
     None: x has P rows that are already in sorted order. Returns (P, N); padding rows and rows of
     an expert id outside [0, E) are zero, rows past num_tokens_post_padded are not written.
     """
-    return torch.ops.w4a8_b200.fp8_block_moe_gemm(
+    return _fp8_block_moe_gemm_op(
         x, x_scales, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded,
         int(top_k), int(block_m), out_dtype)
 
@@ -235,7 +242,7 @@ def fp8_block_moe_gemm1_silu(x, x_scales, w, w_scales, sorted_token_ids, expert_
     reads for the down product. silu(gate) * up is evaluated in fp32 and rounded once, to e4m3.
     inter must be a multiple of 128; the rest as fp8_block_moe_gemm.
     """
-    q, s = torch.ops.w4a8_b200.fp8_block_moe_gemm1_silu(
+    q, s = _fp8_block_moe_gemm1_silu_op(
         x, x_scales, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded,
         int(top_k), int(block_m))
     return q, s
@@ -310,8 +317,8 @@ if _register_fake is not None:
         M, H = x.shape
         return [x.new_empty((M, H), dtype=torch.float8_e4m3fn),
                 x.new_empty((M, _blocks(H)), dtype=torch.float32),
-                x.new_empty((M, H) if residual is not None else (0,)),
-                x.new_empty((M, H) if with_normed else (0,))]
+                x.new_empty((M if residual is not None else 0, H)),
+                x.new_empty((M if with_normed else 0, H))]
 
     @_register_fake("w4a8_b200::fp8_block_gemm")
     def _fake_fp8_block_gemm(x, x_scales, w, w_scales, out_dtype):

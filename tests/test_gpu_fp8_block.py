@@ -124,7 +124,7 @@ def test_rms_norm_quant_edges(w4):
 def test_rms_norm_quant_residual_in_place(w4):
     """The C entry may be given the residual itself as the new residual."""
     g = _gen(9)
-    for H in (2048, 1000):
+    for H in (2048, 1000, 1001):
         x, r = _randn(g, 17, H, dtype=BF16), _randn(g, 17, H, dtype=BF16)
         w = _randn(g, H, dtype=BF16)
         q, s, res, _ = w4.rms_norm_quant_fp8(x, w, 1e-6, residual=r)
