@@ -14,6 +14,8 @@
 // scale. An infinity makes its block's scale infinite, so that a product over it is not finite.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -73,8 +75,39 @@ struct Vec8 {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
     }
-    __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(w)[i]); }
-    __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(w)[i] = from_f32<T>(v); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(u[i]);
+                v[i + 1] = __uint_as_float(u[i + 1]);
+            } else if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i / 2]));
+                v[i] = f.x;
+                v[i + 1] = f.y;
+            } else {  // a bf16 is the upper half of its fp32
+                v[i] = __uint_as_float(u[i / 2] << 16);
+                v[i + 1] = __uint_as_float(u[i / 2] & 0xffff0000u);
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+        uint32_t* u = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            if constexpr (sizeof(T) == 4) {
+                u[i] = __float_as_uint(v[i]);
+                u[i + 1] = __float_as_uint(v[i + 1]);
+            } else if constexpr (std::is_same<T, __half>::value) {
+                const __half2 h = __floats2half2_rn(v[i], v[i + 1]);
+                u[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
+                u[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+    }
 };
 
 // e4m3 bytes of v / s, IEEE quotients. With r the correctly rounded reciprocal of s and y = v r,
@@ -84,31 +117,43 @@ struct Vec8 {
 // Where the residual underflows, the quotient is far below e4m3's smallest value.
 __device__ __forceinline__ float quotient(float v, float s, float r) {
     const float y = __fmul_rn(v, r);
-    return copysignf(__fmaf_rn(__fmaf_rn(-y, s, v), r, y), v);  // -0 has no residual to keep its sign
+    return __fmaf_rn(__fmaf_rn(-y, s, v), r, y);
 }
 
+// max(amax, floor) / 448, the IEEE quotient.
+__device__ __forceinline__ float scale_of(float amax) {
+    const float a = fmaxf(amax, kAmaxFloor);
+    return isinf(a) ? a : quotient(a, kE4m3Max, 1.f / kE4m3Max);
+}
+
+// kSign: zeros keep their sign (the residual of a -0 is +0).
+template <bool kSign>
 __device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale) {
     const float r = __frcp_rn(scale), s = isinf(scale) ? 0.f : scale;
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = quotient(v[i], s, r);
+    for (int i = 0; i < 8; ++i) {
+        y[i] = quotient(v[i], s, r);
+        if (kSign) y[i] = copysignf(y[i], v[i]);
+    }
     return make_uint2((uint32_t)f32x2_to_e4m3x2(y[0], y[1]) | (uint32_t)f32x2_to_e4m3x2(y[2], y[3]) << 16,
                       (uint32_t)f32x2_to_e4m3x2(y[4], y[5]) | (uint32_t)f32x2_to_e4m3x2(y[6], y[7]) << 16);
 }
 
 // 16 lanes quantise one block, 8 values each (zeros past the row's end).
+template <bool kSign>
 __device__ __forceinline__ uint2 quant_block_half(const float (&v)[8], float& s) {
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-    amax = lanes_max<16>(amax);
-    s = __fdiv_rn(fmaxf(amax, kAmaxFloor), kE4m3Max);
-    return quant8(v, s);
+    s = scale_of(lanes_max<16>(amax));
+    return quant8<kSign>(v, s);
 }
 
 // K % 8 == 0 and aligned rows: 16 lanes per block, kPerHalf blocks each, all requested first.
+// kFull: K % 128 == 0, where blocks follow one another in memory and need no row arithmetic.
 constexpr int kPerHalf = 4;
-template <typename T>
+template <typename T, bool kFull>
 __global__ void __launch_bounds__(256)
 act_quant_block_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                            float* __restrict__ scales, int64_t blocks, uint32_t K, uint32_t G) {
@@ -119,26 +164,27 @@ act_quant_block_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
 #pragma unroll
     for (int i = 0; i < kPerHalf; ++i) {
         const int64_t b = b0 + i * 16;
-        at[i] = -1;
-        x8[i].zero();
-        if (b < blocks) {
+        bool ok = b < blocks;
+        if (kFull) {
+            at[i] = (b0 * kBlk + sub * 8) + i * 16 * kBlk;
+        } else {
             const int64_t r = blocks <= INT32_MAX ? (int64_t)((uint32_t)b / G) : b / G;
             const uint32_t k = (uint32_t)(b - r * G) * kBlk + sub * 8;
-            if (k < K) {
-                at[i] = r * K + k;
-                x8[i].load(x + at[i]);
-            }
+            at[i] = r * K + k;
+            ok = ok && k < K;
         }
+        x8[i].zero();
+        if (ok) x8[i].load(x + at[i]);
+        if (!kFull && !ok) at[i] = -1;
     }
 #pragma unroll
     for (int i = 0; i < kPerHalf; ++i) {
         const int64_t b = b0 + i * 16;
         float v[8], s;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = x8[i].get(j);
-        const uint2 u = quant_block_half(v, s);
+        x8[i].get(v);
+        const uint2 u = quant_block_half<true>(v, s);
         if (sub == 0 && b < blocks) scales[b] = s;
-        if (at[i] >= 0) *reinterpret_cast<uint2*>(q + at[i]) = u;
+        if (kFull ? b < blocks : at[i] >= 0) *reinterpret_cast<uint2*>(q + at[i]) = u;
     }
 }
 
@@ -176,17 +222,20 @@ rms_norm_quant_vec_kernel(const T* __restrict__ x, const T* residual, const W* _
         float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+            float h[8];
+            x8[j].get(h);
             if (residual) {
+                float d[8];
+                r8[j].get(d);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x8[j].set(i, x8[j].get(i) + r8[j].get(i));
+                for (int i = 0; i < 8; ++i) h[i] += d[i];
+                x8[j].set(h);
+                x8[j].get(h);
                 const uint32_t n = j * kThreads + tid;
                 if (n < vecs) x8[j].store(residual_out + base + n * 8);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float h = x8[j].get(i);
-                ss += h * h;
-            }
+            for (int i = 0; i < 8; ++i) ss += h[i] * h[i];
         }
         ss = warp_sum(ss);
         if (lane == 0) part[turn][warp] = ss;
@@ -198,16 +247,21 @@ rms_norm_quant_vec_kernel(const T* __restrict__ x, const T* residual, const W* _
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t n = j * kThreads + tid;
-            float v[8], s;
+            float v[8], wv[8], s;
+            x8[j].get(v);  // zeros past the row's end
+            w8[j].get(wv);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = n < vecs ? x8[j].get(i) * rstd * w8[j].get(i) : 0.f;
-            const uint2 u = quant_block_half(v, s);
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * rstd * wv[i];
+            if (n >= vecs) {  // 0 * rstd is NaN in a row that overflowed
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = 0.f;
+            }
+            const uint2 u = quant_block_half<false>(v, s);
             if (n < vecs) {
                 if ((tid & 15) == 0) scales[r * G + n / 16] = s;
                 *reinterpret_cast<uint2*>(q + base + n * 8) = u;
                 if (normed) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x8[j].set(i, v[i]);
+                    x8[j].set(v);
                     x8[j].store(normed + base + n * 8);
                 }
             }
@@ -306,8 +360,12 @@ int launch_quant(const void* x, int64_t M, int64_t K, uint8_t* q, float* scales,
     if (K % 8 == 0 && aligned(x, 16) && aligned(q, 8)) {
         const int64_t ctas = (blocks + 16 * kPerHalf - 1) / (16 * kPerHalf);
         if (ctas <= INT32_MAX) {
-            act_quant_block_vec_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(
-                static_cast<const T*>(x), q, scales, blocks, (uint32_t)K, (uint32_t)G);
+            if (K % kBlk == 0)
+                act_quant_block_vec_kernel<T, true><<<(unsigned)ctas, 256, 0, st>>>(
+                    static_cast<const T*>(x), q, scales, blocks, (uint32_t)K, (uint32_t)G);
+            else
+                act_quant_block_vec_kernel<T, false><<<(unsigned)ctas, 256, 0, st>>>(
+                    static_cast<const T*>(x), q, scales, blocks, (uint32_t)K, (uint32_t)G);
             return launch_status();
         }
     }
