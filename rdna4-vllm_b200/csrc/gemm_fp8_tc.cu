@@ -15,13 +15,19 @@
 //              in the 128-byte swizzle that the MMA's K-major descriptors read.
 //   warp 1     owns tensor memory; one thread issues 4 x tcgen05.mma.kind::f8f6f4 (K = 32) per
 //              block into a ring of fp32 accumulators (512 / BN of them).
-//   warps 10, 11  copy the x rows of tall routed tiles (64 or 128 rows) with cp.async instead.
-//   warps 2-9  fold: lane quarter warp % 4, one half of the columns each; then the epilogue.
+//   warps 2, 3 copy the x rows of tall routed tiles (64 or 128 rows) with cp.async instead.
+//   warps 4-11 fold: lane quarter warp % 4, one half of the columns each; then the epilogue. They
+//              take the registers that the first four warps give back (setmaxnreg; 128 x 56 +
+//              256 x 224 = 384 x 168, what the block was launched with).
 //
 // When there are fewer tiles than SMs, a cluster of S CTAs shares a tile: each takes a slice of
 // the K blocks, parks its fp32 partial tile in shared memory, and after a cluster barrier CTA r
 // sums rows r, r + S, ... over the cluster in rank order (distributed shared memory), so the
 // result does not depend on timing.
+//
+// What bounds it. A block of a 128 x 256 tile is 512 cycles of MMA at the tensor cores' rate, but
+// the shared memory takes 96 KB of traffic for it (48 KB written by TMA, 48 KB read by the MMA),
+// 768 cycles; measured, a thread that issues one block after another is held up for 770.
 //
 // Every mbarrier wait is bounded (sm100.cuh). When one gives up, the CTA stops waiting, waits
 // (boundedly) for its own copies in flight, writes NaN to the tile's outputs and frees tensor
@@ -44,7 +50,8 @@ namespace {
 
 constexpr int kBlk = 128;
 constexpr int kThreads = 384;
-constexpr int kGatherWarps = 2;  // warps 10 and 11
+constexpr int kGatherWarps = 2;  // warps 2 and 3
+constexpr int kFoldWarp0 = 4;    // warps 4 to 11 fold
 constexpr int kFoldWarps = 8;
 constexpr int kMaxSplit = 8;
 
@@ -71,6 +78,7 @@ struct Smem {
     uint8_t stage_out[C::kLive][C::kLines][4096];
     uint64_t full[C::kStages], empty[C::kStages];
     uint64_t tfull[C::kAcc], tempty[C::kAcc];
+    int src[TR];  // x's rows of the gather warps' tile, -1 for none
     uint32_t tmem_base;
     int bad;
     static_assert(C::kABytes + C::kBBytes >= 128 * 128, "the x operand's reads stay in the ring");
@@ -86,7 +94,7 @@ struct TcArgs {
     int tile_rows;  // 16, 32, 64 or 128 rows of x per tile
     int split;      // CTAs per cluster
     int n_tiles;    // weight tiles per row block
-    int out_tma;    // out's rows are TMA-storable: 16-byte aligned base and pitch
+    int out_tma;    // out's rows are 16-byte aligned, as TMA stores and 16-byte stores need them
 };
 
 template <int N>
@@ -135,6 +143,19 @@ __device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// Whether a phase is complete, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 // Waits for the loads into v; the operands keep every use of v behind the wait.
 __device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -143,6 +164,32 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
                    "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
                  :
                  : "memory");
+}
+
+// One block's accumulator into the running totals: columns col(0..kCols) at `base`, the first half
+// scaled by f0 and the second by f1.
+template <int kCols, typename Col>
+__device__ __forceinline__ void fold_block(uint32_t base, Col col, float f0, float f1,
+                                           float (&tot)[kCols]) {
+    uint32_t v[2][16];
+    tmem_ld16_nowait(base + col(0), v[0]);
+    tmem_wait16(v[0]);
+#pragma unroll
+    for (int j = 0; j < kCols; j += 16) {
+        uint32_t(&now)[16] = v[(j / 16) & 1];
+        uint32_t(&next)[16] = v[(j / 16 + 1) & 1];
+        if (j + 16 < kCols) tmem_ld16_nowait(base + col(j + 16), next);
+        const float f = j < kCols / 2 ? f0 : f1;
+        const float2 f2 = make_float2(f, f);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float2 acc = make_float2(__uint_as_float(now[i]), __uint_as_float(now[i + 1]));
+            const float2 p = ffma2(acc, f2, make_float2(tot[j + i], tot[j + i + 1]));
+            tot[j + i] = p.x;
+            tot[j + i + 1] = p.y;
+        }
+        if (j + 16 < kCols) tmem_wait16(next);
+    }
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -165,10 +212,16 @@ __device__ __forceinline__ float4 ld_cluster(const float* p, uint32_t rank) {
     return v;
 }
 
-// silu(g) * u with the fast exponential and quotient, together within 10 units of 2^-24 plus
-// |g| 2^-24 from the exponential's argument: below the product sums' own error.
-__device__ __forceinline__ float silu_mul(float g, float u) {
-    return __fdividef(g, 1.f + __expf(-g)) * u;
+// silu(g) * u of two outputs, g0 and u0 replaced by the results. One reciprocal serves both
+// denominators d = 1 + exp(-g), 1 / d0 = d1 / (d0 d1): the special-function unit, at 16 a cycle
+// and SM, is what this step waits for. exp(-g) is cut at 2^62 to keep the product in range (silu
+// is below 2^-56 there). Together within 12 units of 2^-24, plus |g| 2^-24 from the exponential's
+// argument: below the product sums' own error.
+__device__ __forceinline__ void silu_mul2(float& g0, float& g1, float u0, float u1) {
+    const float d0 = 1.f + fminf(__expf(-g0), 0x1p62f), d1 = 1.f + fminf(__expf(-g1), 0x1p62f);
+    const float r = __fdividef(1.f, d0 * d1);
+    g0 = g0 * u0 * (d1 * r);
+    g1 = g1 * u1 * (d0 * r);
 }
 
 // Four e4m3 bytes of v / scale, rcp = 1 / scale. The values carry more than the 2^-23 by which the
@@ -192,19 +245,11 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Outputs of one row from column n on, held in 16 bytes (8 of 16 bits, 4 of fp32).
-template <int size>
-__device__ __forceinline__ void store16(const Fp8Args& a, bool vec, int64_t r, int64_t n, uint4 v) {
-    constexpr int per = 16 / size;
-    uint8_t* p = static_cast<uint8_t*>(a.out) + (r * a.N + n) * size;
-    if (vec && n + per <= a.N) {
-        *reinterpret_cast<uint4*>(p) = v;
-        return;
-    }
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(&v);
-#pragma unroll 1
-    for (int i = 0; i < (int)min((int64_t)per, a.N - n) * size / 2; ++i)
-        reinterpret_cast<uint16_t*>(p)[i] = h[i];
+// 32 bytes of one row: a whole sector per lane, so that rows need no regrouping between lanes.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&u)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0]), "r"(u[1]),
+                 "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
 }
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
@@ -220,32 +265,23 @@ __device__ __forceinline__ void staging_free() {
     __syncwarp();
 }
 
-// Fills the lane's row of the staged lines.
-__device__ __forceinline__ void refill_row(uint8_t* so, int lines, uint32_t v) {
-    uint8_t* p = so + (threadIdx.x & 31) * 128;
-#pragma unroll 1
-    for (int i = 0; i < lines * 8; ++i)
-        *reinterpret_cast<uint4*>(p + (i >> 3) * 4096 + (i & 7) * 16) = make_uint4(v, v, v, v);
-}
-
 // Sends a warp's staged lines (32 rows x 128 bytes, 16-byte chunks XORed with row % 8, the
 // 128-byte swizzle) to rows r_first + [0, box_rows) and columns n_first on. `whole`: the box may
 // be stored as it is; else only rows below `rows` are, by plain stores.
 template <int size>
 __device__ __forceinline__ void send_lines(const TcArgs& t, const CUtensorMap* tmo, uint8_t* so,
-                                           int lines, int64_t r_first, int64_t rows, int64_t n_first,
+                                           int lines, int r_first, int64_t rows, int n_first,
                                            bool whole) {
     const Fp8Args& a = t.f;
+    constexpr int per = 128 / size;  // columns of a line
     const int lane = threadIdx.x & 31;
-    constexpr int per = 128 / size;
-    const int box_rows = min(t.tile_rows, 32);
     if (t.out_tma && whole) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
             for (int l = 0; l < lines; ++l)
                 if (n_first + l * per < a.N)
-                    tma_store_2d(tmo, (int)(n_first + l * per) * size, (int)r_first, so + l * 4096);
+                    tma_store_2d(tmo, (n_first + l * per) * size, r_first, so + l * 4096);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
         return;
@@ -254,10 +290,21 @@ __device__ __forceinline__ void send_lines(const TcArgs& t, const CUtensorMap* t
 #pragma unroll 1
     for (int i = 0; i < lines * 8; ++i) {
         const int rr = (i & 7) * 4 + (lane >> 3), line = i >> 3;
-        const uint4 u = *reinterpret_cast<const uint4*>(so + line * 4096 + rr * 128 +
+        const uint4 v = *reinterpret_cast<const uint4*>(so + line * 4096 + rr * 128 +
                                                         (((lane & 7) ^ (rr & 7)) << 4));
-        const int64_t n = n_first + line * per + (lane & 7) * (per / 8);
-        if (rr < box_rows && r_first + rr < rows && n < a.N) store16<size>(a, t.out_tma, r_first + rr, n, u);
+        const int64_t r = (int64_t)r_first + rr;
+        const int n = n_first + line * per + (lane & 7) * (per / 8);
+        if (rr >= min(t.tile_rows, 32) || r >= rows || n >= a.N) continue;
+        uint8_t* p = static_cast<uint8_t*>(a.out) + (r * a.N + n) * size;
+        if (t.out_tma) {  // 16-byte aligned rows
+            *reinterpret_cast<uint4*>(p) = v;
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(&v);
+            const int left = (int)min((int64_t)(per / 8), a.N - n) * size / 2;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < left) reinterpret_cast<uint16_t*>(p)[k] = h[k];
+        }
     }
 }
 
@@ -313,415 +360,422 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     asm volatile("tcgen05.fence::after_thread_sync;" ::);
     const uint32_t tmem = sm.tmem_base;
 
-    // One pass runs all of the CTA's tiles, every role at its own pace; with a split, one tile,
-    // and the cluster meets before the next.
-    Ring<C::kStages> st;  // stage ring position of the producer and of the MMA issuer
-    Ring<C::kAcc> tb;     // accumulator ring position of the MMA issuer and of the fold
+    // One pass runs all of the CTA's tiles, every role at its own pace; with a split it is one tile,
+    // and the cluster meets before the next. Each role keeps its ring positions over the passes.
     uint32_t issued = 0;
     Walk cur = first;
-    do {
-    if (warp == 0) {
-        // ---------------- TMA producer ----------------
-        const uint32_t stage_bytes = (copy_rows ? 0u : (uint32_t)t.tile_rows * 128) + C::kBBytes;
-        for (Walk w = cur; w.more(); w.next()) {
-            const int e = expert_of(w.rb);
-            if (e < 0 || e >= a.E) {
-                if (SPLIT) break;
-                continue;
-            }
-            const int r0 = w.rb * t.tile_rows;
-            int src[4] = {0, 0, 0, 0};  // gathered rows 4 * lane + i; padding rows read row 0
-            if (tma_gather && 4 * lane < t.tile_rows)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    src[i] = (int)max((int64_t)0, source_row(a, r0 + 4 * lane + i, rows, e));
-            const int w_row = (int)(e * a.N) + w.nt * n_step;
-            for (int g = g_lo; g < g_hi; ++g) {
-                uint8_t* xa = sm.ring[st.idx];
-                uint64_t* fb = &sm.full[st.idx];
-                if (lane == 0) {
-                    mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
-                    mbar_expect_tx(fb, stage_bytes);
-                    uint8_t* wb = xa + C::kABytes;
-                    tma_load_2d(wb, &tmw, g * 128, w_row, fb);
-                    if (BN == 256)
-                        tma_load_2d(wb + 128 * 128, &tmw, g * 128,
-                                    SILU ? w_row + (int)(a.N / 2) : w_row + 128, fb);
-                    if (!a.sorted_ids) tma_load_2d(xa, &tmx, g * 128, r0, fb);
-                }
-                __syncwarp();
-                if (tma_gather && 4 * lane < t.tile_rows)
-                    tma_gather4(xa + lane * 512, &tmx, g * 128, src, fb);
-                st.next();
-                ++issued;
-            }
-            if (SPLIT) break;
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        if (lane == 0) {
-            constexpr uint32_t idesc = umma_idesc(128, BN);
-            for (Walk w = cur; w.more(); w.next()) {
-                const int e = expert_of(w.rb);
-                if (e < 0 || e >= a.E) {
-                    if (SPLIT) break;
-                    continue;
-                }
-                for (int g = g_lo; g < g_hi; ++g) {
-                    mbar_wait(&sm.full[st.idx], st.phase, bad);
-                    mbar_wait(&sm.tempty[tb.idx], tb.phase ^ 1, bad);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::);
-                    const uint32_t xa = smem_u32(sm.ring[st.idx]);
-                    const uint32_t d = tmem + tb.idx * BN;
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t da = desc_sw128(xa + kk * 32);
-                        const uint64_t db = desc_sw128(xa + C::kABytes + kk * 32);
-                        asm volatile(
-                            "{\n\t.reg .pred p;\n\t"
-                            "setp.ne.b32 p, %4, 0;\n\t"
-                            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                            "l"(da), "l"(db), "r"(idesc), "r"(kk > 0 ? 1u : 0u));
+    if (warp < kFoldWarp0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        Ring<C::kStages> st;
+        Ring<C::kAcc> tb;
+        do {
+            if (warp == 0) {
+                // ---------------- TMA producer ----------------
+                const uint32_t stage_bytes = (copy_rows ? 0u : (uint32_t)t.tile_rows * 128) + C::kBBytes;
+                for (Walk w = cur; w.more(); w.next()) {
+                    const int e = expert_of(w.rb);
+                    if (e < 0 || e >= a.E) {
+                        if (SPLIT) break;
+                        continue;
                     }
-                    asm volatile(
-                        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                        ::"r"(smem_u32(&sm.empty[st.idx])));
-                    asm volatile(
-                        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                        ::"r"(smem_u32(&sm.tfull[tb.idx])));
-                    st.next();
-                    tb.next();
-                }
-                if (SPLIT) break;
-            }
-        }
-        __syncwarp();
-    } else if (warp >= 2 + kFoldWarps) {
-        // ---------------- gather warps: x rows in routing order, tall tiles ----------------
-        // Lane l copies 16-byte chunk l % 8 of rows (l / 8) + 4 (warp index) + 8 i; a stage is
-        // announced when the next one has been requested, so that two are in flight.
-        if (copy_rows) {
-            constexpr int kRowsPer = TR / (4 * kGatherWarps);
-            const int chunk = lane & 7, row0 = (warp - 2 - kFoldWarps) * 4 + (lane >> 3);
-            int pending = -1;  // stage requested but not announced
-            auto announce = [&](int stage) {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.full[stage]);
-            };
-            int slot[kRowsPer], e = -1;  // of the tile to enter next, fetched a tile ahead
-            auto look = [&](const Walk& w) {
-                if (!w.more()) return;
-                e = expert_of(w.rb);
+                    const int r0 = w.rb * t.tile_rows;
+                    int src[4] = {0, 0, 0, 0};  // gathered rows 4 * lane + i; padding rows read row 0
+                    if (tma_gather && 4 * lane < t.tile_rows)
 #pragma unroll
-                for (int i = 0; i < kRowsPer; ++i) {
-                    const int tr = row0 + i * 4 * kGatherWarps;
-                    const int64_t r = (int64_t)w.rb * t.tile_rows + tr;
-                    slot[i] = tr < t.tile_rows && r < rows ? a.sorted_ids[r] : -1;
-                }
-            };
-            Walk w = cur;
-            look(w);
-            while (w.more()) {
-                const bool present = e >= 0 && e < a.E;
-                int src[kRowsPer];
-#pragma unroll
-                for (int i = 0; i < kRowsPer; ++i)
-                    src[i] = slot[i] >= 0 && slot[i] < a.num_slots ? slot[i] / a.top_k : -1;
-                w.next();
-                if (!SPLIT) look(w);
-                if (!present) {
-                    if (SPLIT) break;
-                    continue;
-                }
-                for (int g = g_lo; g < g_hi; ++g) {
-                    mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
-                    const int64_t k = (int64_t)g * kBlk + chunk * 16;
-                    const uint32_t xa = smem_u32(sm.ring[st.idx]);
-#pragma unroll
-                    for (int i = 0; i < kRowsPer; ++i) {
-                        const int tr = row0 + i * 4 * kGatherWarps;
-                        if (tr >= t.tile_rows) break;
-                        // absent rows and columns past K are written as zeros (source size 0)
-                        const bool ok = src[i] >= 0 && k < a.K;
-                        const uint8_t* p = a.x + (ok ? (int64_t)src[i] * a.K + k : 0);
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                         xa + tr * 128 + ((chunk ^ (tr & 7)) << 4)),
-                                     "l"(p), "r"(ok ? 16 : 0)
-                                     : "memory");
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    if (pending >= 0) {
-                        asm volatile("cp.async.wait_group 1;" ::: "memory");
-                        announce(pending);
-                    }
-                    pending = (int)st.idx;
-                    st.next();
-                }
-                if (SPLIT) break;
-            }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (pending >= 0) announce(pending);
-        }
-        __syncwarp();
-    } else {
-        // ---------------- fold + epilogue ----------------
-        const int q = warp & 3, fw = warp - 2, half = fw >> 2;
-        const int row = q * 32 + lane;
-        if (q * 32 < t.tile_rows) {
-            // column of tot[j]: the plain form's half is contiguous; the SiLU form's holds 64
-            // gate columns, then the 64 matching up columns
-            auto col = [&](int j) {
-                return SILU ? (j < 64 ? half * 64 + j : 128 + half * 64 + j - 64) : half * C::kCols + j;
-            };
-            const int64_t NB = (a.N + kBlk - 1) / kBlk;
-            int done = 0;
-            // The scales of a tile's first block are fetched while the tile before it folds its
-            // last one, its routing entries a whole tile ahead: neither wait is paid per tile.
-            const float *xs = a.xs, *ws0 = a.ws, *ws1 = a.ws;
-            float sx = 0.f, s0 = 0.f, s1 = 0.f;
-            bool present = false, dead = true;  // of tile w, set by enter()
-            int next_e = -1, next_slot = -1;    // of the tile to enter next
-            auto look = [&](const Walk& w) {
-                if (!w.more()) return;
-                const int64_t r = (int64_t)w.rb * t.tile_rows + row;
-                next_e = expert_of(w.rb);
-                next_slot = row >= t.tile_rows || r >= rows ? -1 : a.sorted_ids ? a.sorted_ids[r] : (int)r;
-            };
-            auto enter = [&](const Walk& w) {
-                const int e = next_e;
-                present = e >= 0 && e < a.E;
-                int src = next_slot;
-                if (a.sorted_ids) src = src >= 0 && src < a.num_slots ? src / a.top_k : -1;
-                dead = !present || src < 0;
-                if (!present) return;
-                const int64_t n0 = (int64_t)w.nt * n_step;
-                const int64_t b0 = SILU ? n0 / kBlk : min((n0 + half * C::kCols) / kBlk, NB - 1);
-                xs = a.xs + (int64_t)max(src, 0) * G;
-                ws0 = a.ws + (e * NB + b0) * G;
-                ws1 = SILU ? ws0 + (a.N / 2 / kBlk) * G : ws0;
-                if (g_lo < g_hi) {
-                    sx = __ldg(xs + g_lo);
-                    s0 = __ldg(ws0 + g_lo);
-                    if (SILU) s1 = __ldg(ws1 + g_lo);
-                }
-            };
-            Walk w = cur;
-            look(w);
-            if (w.more()) enter(w);
-            while (w.more()) {
-                const int64_t r0 = (int64_t)w.rb * t.tile_rows, r = r0 + row;
-                const int64_t n0 = (int64_t)w.nt * n_step;
-                const bool is_dead = dead, is_present = present && g_lo < g_hi;
-                w.next();
-                if (!SPLIT) look(w);
-                float tot[C::kCols];
-#pragma unroll
-                for (int j = 0; j < C::kCols; ++j) tot[j] = 0.f;
-                if (!is_present && !SPLIT && w.more()) enter(w);
-                if (is_present) {
+                        for (int i = 0; i < 4; ++i)
+                            src[i] = (int)max((int64_t)0, source_row(a, r0 + 4 * lane + i, rows, e));
+                    const int w_row = (int)(e * a.N) + w.nt * n_step;
                     for (int g = g_lo; g < g_hi; ++g) {
-                        const float f0 = sx * s0, f1 = SILU ? sx * s1 : f0;
-                        if (g + 1 < g_hi) {  // the next block's scales, behind this block's fold
-                            sx = __ldg(xs + g + 1);
-                            s0 = __ldg(ws0 + g + 1);
-                            if (SILU) s1 = __ldg(ws1 + g + 1);
-                        } else if (!SPLIT && w.more()) {
-                            enter(w);
+                        uint8_t* xa = sm.ring[st.idx];
+                        uint64_t* fb = &sm.full[st.idx];
+                        if (lane == 0) {
+                            mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
+                            mbar_expect_tx(fb, stage_bytes);
+                            uint8_t* wb = xa + C::kABytes;
+                            tma_load_2d(wb, &tmw, g * 128, w_row, fb);
+                            if (BN == 256)
+                                tma_load_2d(wb + 128 * 128, &tmw, g * 128,
+                                            SILU ? w_row + (int)(a.N / 2) : w_row + 128, fb);
+                            if (!a.sorted_ids) tma_load_2d(xa, &tmx, g * 128, r0, fb);
                         }
-                        mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::);
-                        const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + tb.idx * BN;
-                        uint32_t v[2][16];
-                        tmem_ld16_nowait(base + col(0), v[0]);
-                        tmem_wait16(v[0]);
-#pragma unroll
-                        for (int j = 0; j < C::kCols; j += 16) {
-                            uint32_t(&now)[16] = v[(j / 16) & 1];
-                            uint32_t(&nxt)[16] = v[(j / 16 + 1) & 1];
-                            if (j + 16 < C::kCols) tmem_ld16_nowait(base + col(j + 16), nxt);
-                            const float f = j < C::kCols / 2 ? f0 : f1;
-                            const float2 f2 = make_float2(f, f);
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const float2 p = ffma2(
-                                    make_float2(__uint_as_float(now[i]), __uint_as_float(now[i + 1])),
-                                    f2, make_float2(tot[j + i], tot[j + i + 1]));
-                                tot[j + i] = p.x;
-                                tot[j + i + 1] = p.y;
-                            }
-                            if (j + 16 < C::kCols) tmem_wait16(nxt);
-                        }
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::);
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sm.tempty[tb.idx]);
-                        tb.next();
+                        if (tma_gather && 4 * lane < t.tile_rows)
+                            tma_gather4(xa + lane * 512, &tmx, g * 128, src, fb);
+                        st.next();
+                        ++issued;
+                    }
+                    if (SPLIT) break;
+                }
+                __syncwarp();
+            } else if (warp == 1) {
+                // ---------------- MMA issuer ----------------
+                if (lane == 0) {
+                    constexpr uint32_t idesc = umma_idesc(128, BN);
+                    bool full = false, room = false;  // the next block's barriers were seen complete
+                    for (Walk w = cur; w.more(); w.next()) {
+                        const int e = expert_of(w.rb);
+                        if (e < 0 || e >= a.E) {
+                            if (SPLIT) break;
+                            continue;
+                        }
+                        for (int g = g_lo; g < g_hi; ++g) {
+                            if (!full) mbar_wait(&sm.full[st.idx], st.phase, bad);
+                            if (!room) mbar_wait(&sm.tempty[tb.idx], tb.phase ^ 1, bad);
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::);
+                            const uint32_t xa = smem_u32(sm.ring[st.idx]);
+                            const uint32_t d = tmem + tb.idx * BN;
+                            const uint32_t stage_done = smem_u32(&sm.empty[st.idx]);
+                            const uint32_t acc_done = smem_u32(&sm.tfull[tb.idx]);
+                            st.next();
+                            tb.next();
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                // while MMAs are queued, a look at the next block's barriers is free
+                                if (kk == 3) {
+                                    full = mbar_test(&sm.full[st.idx], st.phase);
+                                    room = mbar_test(&sm.tempty[tb.idx], tb.phase ^ 1);
+                                }
+                                const uint64_t da = desc_sw128(xa + kk * 32);
+                                const uint64_t db = desc_sw128(xa + C::kABytes + kk * 32);
+                                asm volatile(
+                                    "{\n\t.reg .pred p;\n\t"
+                                    "setp.ne.b32 p, %4, 0;\n\t"
+                                    "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                                    "l"(da), "l"(db), "r"(idesc), "r"(kk > 0 ? 1u : 0u));
+                            }
+                            asm volatile(
+                                "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                                ::"r"(stage_done));
+                            asm volatile(
+                                "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                                ::"r"(acc_done));
+                        }
+                        if (SPLIT) break;
                     }
                 }
-                // rows of zeros are zero whatever the lane's accumulator held: such a lane writes
-                // `fill` over its staged row (a wait that gave up makes every row one, of NaN)
-                const bool refill = is_dead || *bad;
-                const float fill = *bad ? __int_as_float(0x7fffffff) : 0.f;
-                if (SPLIT) {
-                    // park the partial tile; the ring is idle once the last accumulator was read
-                    if (row < t.tile_rows) {
-                        float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
+                __syncwarp();
+            } else if (TR == 128 && copy_rows) {
+                // ---------------- gather warps: x rows in routing order, tall tiles ----------------
+                // Lane l copies 16-byte chunk l % 8 of rows (l / 8) + 4 (warp index) + 8 i; a stage is
+                // announced when the next one has been requested, so that two are in flight.
+                if (copy_rows) {
+                    constexpr int kRowsPer = TR / (4 * kGatherWarps);
+                    const int chunk = lane & 7, row0 = (warp - 2) * 4 + (lane >> 3);
+                    int pending = -1;  // stage requested but not announced
+                    auto announce = [&](int stage) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.full[stage]);
+                    };
+                    // the routing entries of the tile to enter next, fetched a tile ahead: lane l
+                    // holds this warp's rows l and l + 32 (of 64), the rows of warp 2 + (row / 4) % 2
+                    int slot[2] = {-1, -1}, e = -1;
+                    auto row_of = [&](int i) { return (i >> 2) * 8 + (warp - 2) * 4 + (i & 3); };
+                    auto look = [&](const Walk& w) {
+                        if (!w.more()) return;
+                        e = expert_of(w.rb);
 #pragma unroll
-                        for (int j = 0; j < C::kCols; j += 4)
-                            *reinterpret_cast<float4*>(part + col(j)) =
-                                make_float4(tot[j], tot[j + 1], tot[j + 2], tot[j + 3]);
-                        if (refill)
-#pragma unroll 1
-                            for (int j = 0; j < C::kCols; ++j)
-                                part[SILU ? (j & 63) + (j >> 6) * 128 + half * 64 : half * C::kCols + j] = fill;
-                    }
-                } else if constexpr (SILU) {
-                    float m = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 64; ++j) {
-                        tot[j] = silu_mul(tot[j], tot[(j + 64) % C::kCols]);
-                        m = fmaxf(m, fabsf(tot[j]));
-                    }
-                    if (refill) m = fill;
-                    // the row's other 64 outputs are with the warp of the other half
-                    float* amax = reinterpret_cast<float*>(sm.stage_out) + (done & 1) * 256;
-                    amax[half * 128 + row] = m;
-                    asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
-                    m = fmaxf(m, amax[(half ^ 1) * 128 + row]);
-                    const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
-                    const float rcp = __frcp_rn(s);
-                    if (row < t.tile_rows && r < rows) {
-                        const int64_t inter = a.N / 2;
-                        if (half == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
-                        uint4* qp = reinterpret_cast<uint4*>(a.q + r * inter + n0 + half * 64);
-#pragma unroll
-                        for (int j = 0; j < 64; j += 16) {
-                            uint32_t u[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                u[i] = quant4(tot[j + 4 * i], tot[j + 4 * i + 1], tot[j + 4 * i + 2],
-                                              tot[j + 4 * i + 3], rcp);
-                            qp[j / 16] = make_uint4(u[0], u[1], u[2], u[3]);
+                        for (int i = 0; i < 2; ++i) {
+                            const int tr = row_of(lane + 32 * i);
+                            const int64_t r = (int64_t)w.rb * t.tile_rows + tr;
+                            slot[i] = tr < t.tile_rows && r < rows ? a.sorted_ids[r] : -1;
                         }
-                        if (refill) {
-                            const uint32_t z = fill == 0.f ? 0u : 0x7f7f7f7fu;
-#pragma unroll 1
-                            for (int j = 0; j < 4; ++j) qp[j] = make_uint4(z, z, z, z);
+                    };
+                    Walk w = cur;
+                    look(w);
+                    while (w.more()) {
+                        const bool present = e >= 0 && e < a.E;
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            sm.src[row_of(lane + 32 * i)] =
+                                slot[i] >= 0 && slot[i] < a.num_slots ? slot[i] / a.top_k : -1;
+                        __syncwarp();
+                        w.next();
+                        if (!SPLIT) look(w);
+                        if (!present) {
+                            if (SPLIT) break;
+                            continue;
+                        }
+                        for (int g = g_lo; g < g_hi; ++g) {
+                            mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
+                            const int64_t k = (int64_t)g * kBlk + chunk * 16;
+                            const uint32_t xa = smem_u32(sm.ring[st.idx]);
+#pragma unroll
+                            for (int i = 0; i < kRowsPer; ++i) {
+                                const int tr = row0 + i * 4 * kGatherWarps;
+                                if (tr >= t.tile_rows) break;
+                                // absent rows and columns past K are written as zeros (source size 0)
+                                const int src = sm.src[tr];
+                                const bool ok = src >= 0 && k < a.K;
+                                const uint8_t* p = a.x + (ok ? (int64_t)src * a.K + k : 0);
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                                 xa + tr * 128 + ((chunk ^ (tr & 7)) << 4)),
+                                             "l"(p), "r"(ok ? 16 : 0)
+                                             : "memory");
+                            }
+                            asm volatile("cp.async.commit_group;" ::: "memory");
+                            if (pending >= 0) {
+                                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                                announce(pending);
+                            }
+                            pending = (int)st.idx;
+                            st.next();
+                        }
+                        if (SPLIT) break;
+                    }
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    if (pending >= 0) announce(pending);
+                }
+                __syncwarp();
+            }
+            if (SPLIT) {
+                cluster_sync();
+                cluster_sync();
+                cur.next();
+            }
+        } while (SPLIT && cur.more());
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        Ring<C::kAcc> tb;
+        do {
+            // ---------------- fold + epilogue ----------------
+            const int q = warp & 3, fw = warp - kFoldWarp0, half = fw >> 2;
+            const int row = q * 32 + lane;
+            if (q * 32 < t.tile_rows) {
+                // column of tot[j]: the plain form's half is contiguous; the SiLU form's holds 64
+                // gate columns, then the 64 matching up columns
+                auto col = [&](int j) {
+                    return SILU ? (j < 64 ? half * 64 + j : 128 + half * 64 + j - 64) : half * C::kCols + j;
+                };
+                const int64_t NB = (a.N + kBlk - 1) / kBlk;
+                int done = 0;
+                // The scales of a tile's first block are fetched while the tile before it folds its
+                // last one, its routing entries a whole tile ahead: neither wait is paid per tile.
+                const float *xs = a.xs, *ws0 = a.ws, *ws1 = a.ws;
+                float sx = 0.f, s0 = 0.f, s1 = 0.f;
+                bool present = false, dead = true;  // of tile w, set by enter()
+                int next_e = -1, next_slot = -1;    // of the tile to enter next
+                auto look = [&](const Walk& w) {
+                    if (!w.more()) return;
+                    const int64_t r = (int64_t)w.rb * t.tile_rows + row;
+                    next_e = expert_of(w.rb);
+                    next_slot = row >= t.tile_rows || r >= rows ? -1 : a.sorted_ids ? a.sorted_ids[r] : (int)r;
+                };
+                auto enter = [&](const Walk& w) {
+                    const int e = next_e;
+                    present = e >= 0 && e < a.E;
+                    int src = next_slot;
+                    if (a.sorted_ids) src = src >= 0 && src < a.num_slots ? src / a.top_k : -1;
+                    dead = !present || src < 0;
+                    if (!present) return;
+                    const int64_t n0 = (int64_t)w.nt * n_step;
+                    const int64_t b0 = SILU ? n0 / kBlk : min((n0 + half * C::kCols) / kBlk, NB - 1);
+                    xs = a.xs + (int64_t)max(src, 0) * G;
+                    ws0 = a.ws + (e * NB + b0) * G;
+                    ws1 = SILU ? ws0 + (a.N / 2 / kBlk) * G : ws0;
+                    if (g_lo < g_hi) {
+                        sx = __ldg(xs + g_lo);
+                        s0 = __ldg(ws0 + g_lo);
+                        if (SILU) s1 = __ldg(ws1 + g_lo);
+                    }
+                };
+                Walk w = cur;
+                look(w);
+                if (w.more()) enter(w);
+                while (w.more()) {
+                    const int64_t r0 = (int64_t)w.rb * t.tile_rows, r = r0 + row;
+                    const int64_t n0 = (int64_t)w.nt * n_step;
+                    const bool is_dead = dead, is_present = present && g_lo < g_hi;
+                    w.next();
+                    if (!SPLIT) look(w);
+                    float tot[C::kCols];
+#pragma unroll
+                    for (int j = 0; j < C::kCols; ++j) tot[j] = 0.f;
+                    if (!is_present && !SPLIT && w.more()) enter(w);
+                    if (is_present) {
+                        for (int g = g_lo; g < g_hi; ++g) {
+                            const float f0 = sx * s0, f1 = SILU ? sx * s1 : f0;
+                            if (g + 1 < g_hi) {  // the next block's scales, behind this block's fold
+                                sx = __ldg(xs + g + 1);
+                                s0 = __ldg(ws0 + g + 1);
+                                if (SILU) s1 = __ldg(ws1 + g + 1);
+                            } else if (!SPLIT && w.more()) {
+                                enter(w);
+                            }
+                            mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::);
+                            fold_block(tmem + ((uint32_t)(q * 32) << 16) + tb.idx * BN, col, f0, f1, tot);
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::);
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sm.tempty[tb.idx]);
+                            tb.next();
                         }
                     }
-                } else {
-                    uint8_t* so = sm.stage_out[TR == 32 ? half : fw][0];
-                    const bool whole = !a.ntp || r0 + q * 32 + min(t.tile_rows, 32) <= rows;
-                    if constexpr (sizeof(Out) == 4) {
+                    // rows of zeros are zero whatever the lane's accumulator held: such a lane writes
+                    // `fill` over its staged row (a wait that gave up makes every row one, of NaN)
+                    const bool refill = is_dead || *bad;
+                    const float fill = *bad ? __int_as_float(0x7fffffff) : 0.f;
+                    if (SPLIT) {
+                        // park the partial tile; the ring is idle once the last accumulator was read
+                        if (row < t.tile_rows) {
+                            float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
 #pragma unroll
-                        for (int c0 = 0; c0 < C::kCols; c0 += C::kCols / 2) {  // 32 columns a line
-                            staging_free();
+                            for (int j = 0; j < C::kCols; j += 4)
+                                *reinterpret_cast<float4*>(part + col(j)) =
+                                    make_float4(tot[j], tot[j + 1], tot[j + 2], tot[j + 3]);
+                            if (refill)
+#pragma unroll 1
+                                for (int j = 0; j < C::kCols; ++j)
+                                    part[SILU ? (j & 63) + (j >> 6) * 128 + half * 64 : half * C::kCols + j] = fill;
+                        }
+                    } else if constexpr (SILU) {
+                        float m = 0.f;
 #pragma unroll
-                            for (int c = 0; c < C::kCols / 2; c += 4)
-                                *reinterpret_cast<float4*>(so + (c / 32) * 4096 + lane * 128 +
-                                                           (((c / 4 % 8) ^ (lane & 7)) << 4)) =
-                                    make_float4(tot[c0 + c], tot[c0 + c + 1], tot[c0 + c + 2],
-                                                tot[c0 + c + 3]);
-                            if (refill) refill_row(so, C::kLines, __float_as_uint(fill));
-                            send_lines<sizeof(Out)>(t, &tmo, so, C::kLines, r0 + q * 32, rows, n0 + col(c0), whole);
+                        for (int j = 0; j < 64; j += 2) {
+                            silu_mul2(tot[j], tot[j + 1], tot[j + 64], tot[j + 65]);
+                            m = fmaxf(m, fmaxf(fabsf(tot[j]), fabsf(tot[j + 1])));
+                        }
+                        if (refill) m = fill;
+                        // the row's other 64 outputs are with the warp of the other half
+                        float* amax = reinterpret_cast<float*>(sm.stage_out) + (done & 1) * 256;
+                        amax[half * 128 + row] = m;
+                        asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
+                        m = fmaxf(m, amax[(half ^ 1) * 128 + row]);
+                        const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
+                        const float rcp = __frcp_rn(s);
+                        if (row < t.tile_rows && r < rows) {
+                            const int64_t inter = a.N / 2;
+                            if (half == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
+                            uint8_t* p = a.q + r * inter + n0 + half * 64;
+#pragma unroll
+                            for (int j = 0; j < 64; j += 32) {
+                                uint32_t u[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    u[i] = quant4(tot[j + 4 * i], tot[j + 4 * i + 1], tot[j + 4 * i + 2],
+                                                  tot[j + 4 * i + 3], rcp);
+                                if (refill)
+#pragma unroll
+                                    for (int i = 0; i < 8; ++i) u[i] = fill == 0.f ? 0u : 0x7f7f7f7fu;
+                                store32(p + j, u);
+                            }
                         }
                     } else {
-                        staging_free();
+                        uint8_t* so = sm.stage_out[TR == 32 ? half : fw][0];
+                        const int r_box = (int)r0 + q * 32;
+                        const bool whole = !a.ntp || r_box + min(t.tile_rows, 32) <= rows;
+                        constexpr int kPass = C::kLines * 128 / sizeof(Out);  // columns per pass
+                        constexpr int kPer = 16 / sizeof(Out);
 #pragma unroll
-                        for (int c = 0; c < C::kCols; c += 8) {  // 64 columns a line
-                            uint4 u;
-                            u.x = pack2<Out>(tot[c], tot[c + 1]);
-                            u.y = pack2<Out>(tot[c + 2], tot[c + 3]);
-                            u.z = pack2<Out>(tot[c + 4], tot[c + 5]);
-                            u.w = pack2<Out>(tot[c + 6], tot[c + 7]);
-                            *reinterpret_cast<uint4*>(so + (c / 64) * 4096 + lane * 128 +
-                                                      (((c / 8 % 8) ^ (lane & 7)) << 4)) = u;
+                        for (int c0 = 0; c0 < C::kCols; c0 += kPass) {
+                            staging_free();
+#pragma unroll
+                            for (int c = 0; c < kPass; c += kPer) {
+                                uint32_t u[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    if constexpr (sizeof(Out) == 4) u[i] = __float_as_uint(tot[c0 + c + i]);
+                                    else u[i] = pack2<Out>(tot[c0 + c + 2 * i], tot[c0 + c + 2 * i + 1]);
+                                }
+                                const int chunk = c / kPer;
+                                *reinterpret_cast<uint4*>(so + (chunk / 8) * 4096 + lane * 128 +
+                                                          (((chunk % 8) ^ (lane & 7)) << 4)) =
+                                    make_uint4(u[0], u[1], u[2], u[3]);
+                            }
+                            if (refill) {
+                                uint32_t v;
+                                if constexpr (sizeof(Out) == 4) v = __float_as_uint(fill);
+                                else v = pack2<Out>(fill, fill);
+#pragma unroll 1
+                                for (int i = 0; i < C::kLines * 8; ++i)
+                                    *reinterpret_cast<uint4*>(so + (i >> 3) * 4096 + lane * 128 + (i & 7) * 16) =
+                                        make_uint4(v, v, v, v);
+                            }
+                            send_lines<sizeof(Out)>(t, &tmo, so, C::kLines, r_box, rows,
+                                                    (int)n0 + col(c0), whole);
                         }
-                        if (refill) refill_row(so, C::kLines, pack2<Out>(fill, fill));
-                        send_lines<sizeof(Out)>(t, &tmo, so, C::kLines, r0 + q * 32, rows, n0 + col(0), whole);
                     }
+                    ++done;
+                    if (SPLIT) break;
                 }
-                ++done;
-                if (SPLIT) break;
+                if (!SPLIT && !SILU && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
-            if (!SILU && !SPLIT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        }
-        __syncwarp();
-    }
-
-    if (SPLIT) {
-        // CTA `rank` finishes rows rank, rank + S, ... of the cluster's tile
-        cluster_sync();
-        if (warp >= 2 && warp < 2 + kFoldWarps && cur.more()) {
-            const int64_t r0 = (int64_t)cur.rb * t.tile_rows, n0 = (int64_t)cur.nt * n_step;
-            const bool vec = t.out_tma;
-            const float* part = reinterpret_cast<const float*>(sm.ring);
-            for (int tr = rank + S * (warp - 2); tr < t.tile_rows; tr += S * kFoldWarps) {
-                const int64_t r = r0 + tr;
-                if (r >= rows) break;
-                float4 sum[BN / 128];
-#pragma unroll
-                for (int c = 0; c < BN / 128; ++c) {
-                    float4 v[kMaxSplit];
-#pragma unroll
-                    for (int k = 0; k < kMaxSplit; ++k)
-                        if (k < S) v[k] = ld_cluster(part + tr * C::kPitch + c * 128 + 4 * lane, k);
-                    sum[c] = v[0];
-#pragma unroll
-                    for (int k = 1; k < kMaxSplit; ++k)
-                        if (k < S) {
-                            sum[c].x += v[k].x;
-                            sum[c].y += v[k].y;
-                            sum[c].z += v[k].z;
-                            sum[c].w += v[k].w;
-                        }
-                }
-                if constexpr (SILU) {
-                    const float4 g4 = sum[0], u4 = sum[BN / 128 - 1];
-                    const float h[4] = {silu_mul(g4.x, u4.x), silu_mul(g4.y, u4.y),
-                                        silu_mul(g4.z, u4.z), silu_mul(g4.w, u4.w)};
-                    float m = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
-                    const float rcp = __frcp_rn(s);
-                    const int64_t inter = a.N / 2;
-                    if (lane == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
-                    *reinterpret_cast<uint32_t*>(a.q + r * inter + n0 + 4 * lane) =
-                        quant4(h[0], h[1], h[2], h[3], rcp);
-                } else {
+            __syncwarp();
+            if (SPLIT) {
+                cluster_sync();
+            // CTA `rank` finishes rows rank, rank + S, ... of the cluster's tile
+            if (cur.more()) {
+                const int64_t r0 = (int64_t)cur.rb * t.tile_rows, n0 = (int64_t)cur.nt * n_step;
+                const bool vec = t.out_tma;
+                const float* part = reinterpret_cast<const float*>(sm.ring);
+                for (int tr = rank + S * (warp - kFoldWarp0); tr < t.tile_rows; tr += S * kFoldWarps) {
+                    const int64_t r = r0 + tr;
+                    if (r >= rows) break;
+                    float4 sum[BN / 128];
 #pragma unroll
                     for (int c = 0; c < BN / 128; ++c) {
-                        const int64_t n = n0 + c * 128 + 4 * lane;
-                        const float o[4] = {sum[c].x, sum[c].y, sum[c].z, sum[c].w};
-                        if constexpr (sizeof(Out) == 4) {
-                            float* p = static_cast<float*>(a.out) + r * a.N + n;
-                            if (vec && n + 4 <= a.N) *reinterpret_cast<float4*>(p) = sum[c];
-                            else
+                        float4 v[kMaxSplit];
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (n + i < a.N) p[i] = o[i];
-                        } else {
-                            uint16_t* p = static_cast<uint16_t*>(a.out) + r * a.N + n;
-                            const uint32_t lo = pack2<Out>(o[0], o[1]);
-                            const uint32_t hi = pack2<Out>(o[2], o[3]);
-                            if (vec && n + 4 <= a.N) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
-                            else
+                        for (int k = 0; k < kMaxSplit; ++k)
+                            if (k < S) v[k] = ld_cluster(part + tr * C::kPitch + c * 128 + 4 * lane, k);
+                        sum[c] = v[0];
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (n + i < a.N) p[i] = (uint16_t)((i < 2 ? lo : hi) >> ((i & 1) * 16));
+                        for (int k = 1; k < kMaxSplit; ++k)
+                            if (k < S) {
+                                sum[c].x += v[k].x;
+                                sum[c].y += v[k].y;
+                                sum[c].z += v[k].z;
+                                sum[c].w += v[k].w;
+                            }
+                    }
+                    if constexpr (SILU) {
+                        const float4 g4 = sum[0], u4 = sum[BN / 128 - 1];
+                        float h[4] = {g4.x, g4.y, g4.z, g4.w};
+                        silu_mul2(h[0], h[1], u4.x, u4.y);
+                        silu_mul2(h[2], h[3], u4.z, u4.w);
+                        float m = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
+                        const float rcp = __frcp_rn(s);
+                        const int64_t inter = a.N / 2;
+                        if (lane == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
+                        *reinterpret_cast<uint32_t*>(a.q + r * inter + n0 + 4 * lane) =
+                            quant4(h[0], h[1], h[2], h[3], rcp);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < BN / 128; ++c) {
+                            const int64_t n = n0 + c * 128 + 4 * lane;
+                            const float o[4] = {sum[c].x, sum[c].y, sum[c].z, sum[c].w};
+                            if constexpr (sizeof(Out) == 4) {
+                                float* p = static_cast<float*>(a.out) + r * a.N + n;
+                                if (vec && n + 4 <= a.N) *reinterpret_cast<float4*>(p) = sum[c];
+                                else
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        if (n + i < a.N) p[i] = o[i];
+                            } else {
+                                uint16_t* p = static_cast<uint16_t*>(a.out) + r * a.N + n;
+                                const uint32_t lo = pack2<Out>(o[0], o[1]);
+                                const uint32_t hi = pack2<Out>(o[2], o[3]);
+                                if (vec && n + 4 <= a.N) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+                                else
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        if (n + i < a.N) p[i] = (uint16_t)((i < 2 ? lo : hi) >> ((i & 1) * 16));
+                            }
                         }
                     }
                 }
             }
-        }
-        // no CTA leaves, or loads its next tile over the parked one, while that is still read
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        cluster_sync();
-        cur.next();
+                // no CTA leaves, or loads its next tile over the parked one, while that is read
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                cluster_sync();
+                cur.next();
+            }
+        } while (SPLIT && cur.more());
     }
-    } while (SPLIT && cur.more());
     // after a wait that gave up: leave no copy in flight
     if (tid == 0 && *bad) {
         const uint64_t t0 = global_ns();
@@ -747,11 +801,11 @@ int sm_count() {
 
 template <int BN, int TR, typename Out, bool SPLIT>
 int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
-    constexpr bool SILU = std::is_void<Out>::value;
     const Fp8Args& a = t.f;
     CUtensorMap tmx, tmw, tmo{};
     const int64_t pitch = a.N * (a.out_dtype == 0 ? 4 : 2);
-    t.out_tma = !SILU && pitch % 16 == 0 && pitch <= INT32_MAX && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+    t.out_tma = !a.silu && pitch % 16 == 0 && pitch <= INT32_MAX &&
+                (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
     if (t.out_tma && !SPLIT &&
         !make_tma_map_u8(&tmo, a.out, (uint64_t)a.P, (uint64_t)pitch, 128, std::min(t.tile_rows, 32),
                          CU_TENSOR_MAP_SWIZZLE_128B))
@@ -804,7 +858,7 @@ int launch_tr(const TcArgs& t, bool bn256, int64_t tiles, cudaStream_t st) {
 bool fp8_tc_ok(const Fp8Args& a) {
     return a.K % 16 == 0 && a.x_rows > 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 &&
            (reinterpret_cast<uintptr_t>(a.w) & 15) == 0 &&
-           (!a.silu || (reinterpret_cast<uintptr_t>(a.q) & 15) == 0);
+           (!a.silu || (reinterpret_cast<uintptr_t>(a.q) & 31) == 0);
 }
 
 int launch_fp8_tc(const Fp8Args& a, cudaStream_t st) {
@@ -823,8 +877,13 @@ int launch_fp8_tc(const Fp8Args& a, cudaStream_t st) {
     const bool bn256 = a.silu || wide >= sms;
     const int64_t tiles = bn256 ? wide : narrow;
     t.n_tiles = (int)(tiles / blocks);
+    // A cluster of 8 (4) finds room on 15 (33) places of the 148 SMs at once, not 18 (37), and a
+    // second round costs more than the wider split gains (16 tiles x 32 blocks of K, M = 128:
+    // 16.9 us with 8, see the commit that limits it).
     t.split = 1;
-    while (t.split < kMaxSplit && tiles * t.split * 2 <= sms && a.G >= t.split * 4) t.split *= 2;
+    const int room[4] = {sms, sms / 2, sms * 33 / 148, sms * 15 / 148};
+    for (int i = 1; i < 4; ++i)
+        if (tiles <= room[i] && a.G >= (2 << i)) t.split = 1 << i;
     return t.tile_rows <= 32 ? launch_tr<32>(t, bn256, tiles, st) : launch_tr<128>(t, bn256, tiles, st);
 }
 
