@@ -17,8 +17,8 @@
 //              block into a ring of fp32 accumulators (512 / BN of them).
 //   warps 2, 3 copy the x rows of tall routed tiles (64 or 128 rows) with cp.async instead.
 //   warps 4-11 fold: lane quarter warp % 4, one half of the columns each; then the epilogue. They
-//              take the registers that the first four warps give back (setmaxnreg; 128 x 56 +
-//              256 x 224 = 384 x 168, what the block was launched with).
+//              take the registers that the first four warps give back (setmaxnreg; 128 x 72 +
+//              256 x 216 = 384 x 168, what the block was launched with).
 //
 // When there are fewer tiles than SMs, a cluster of S CTAs shares a tile: each takes a slice of
 // the K blocks, parks its fp32 partial tile in shared memory, and after a cluster barrier CTA r
@@ -61,11 +61,10 @@ template <int BN, int TR>
 struct Cfg {
     static constexpr uint32_t kABytes = TR * 128;  // a stage's x slab
     static constexpr uint32_t kBBytes = BN * 128;
-    static constexpr int kStages = TR == 32 ? (BN == 256 ? 5 : 10) : (BN == 256 ? 3 : 6);
+    static constexpr int kStages = TR == 32 ? (BN == 256 ? 5 : 10) : (BN == 256 ? 4 : 6);
     static constexpr int kAcc = 512 / BN;
     static constexpr int kCols = BN / 2;           // columns per fold thread
     static constexpr int kLive = TR == 32 ? 2 : kFoldWarps;  // fold warps that may hold rows
-    static constexpr int kLines = kCols / 64;      // staged 128-byte lines per warp and pass
     static constexpr int kPitch = BN + 4;          // floats per row of a parked partial tile
 };
 
@@ -73,9 +72,9 @@ template <int BN, int TR>
 struct Smem {
     using C = Cfg<BN, TR>;
     uint8_t ring[C::kStages][C::kABytes + C::kBBytes];  // 1024-byte aligned
-    // per warp: lines of 32 rows x 128 bytes of finished outputs (1024-byte aligned); the SiLU
-    // form keeps the row maxima of its two column halves here, [tile parity][half][row]
-    uint8_t stage_out[C::kLive][C::kLines][4096];
+    // per warp: 32 rows x 128 bytes of finished outputs; the SiLU form keeps the row maxima of its
+    // two column halves here, [tile parity][half][row]
+    uint8_t stage_out[C::kLive][4096];
     uint64_t full[C::kStages], empty[C::kStages];
     uint64_t tfull[C::kAcc], tempty[C::kAcc];
     int src[TR];  // x's rows of the gather warps' tile, -1 for none
@@ -94,7 +93,7 @@ struct TcArgs {
     int tile_rows;  // 16, 32, 64 or 128 rows of x per tile
     int split;      // CTAs per cluster
     int n_tiles;    // weight tiles per row block
-    int out_tma;    // out's rows are 16-byte aligned, as TMA stores and 16-byte stores need them
+    int out_vec;    // out's rows are 16-byte aligned
 };
 
 template <int N>
@@ -131,6 +130,15 @@ __device__ __forceinline__ int64_t source_row(const Fp8Args& a, int64_t r, int64
     if (!a.sorted_ids) return r;
     const int slot = a.sorted_ids[r];
     return slot >= 0 && slot < a.num_slots ? slot / a.top_k : -1;
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
+                                            uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
 }
 
 __device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x,
@@ -245,74 +253,53 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 32 bytes of one row: a whole sector per lane, so that rows need no regrouping between lanes.
+// 32 bytes of one row.
 __device__ __forceinline__ void store32(void* p, const uint32_t (&u)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0]), "r"(u[1]),
                  "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                  : "memory");
 }
 
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                     reinterpret_cast<uint64_t>(map)),
-                 "r"(x), "r"(y), "r"(smem_u32(src))
-                 : "memory");
-}
-
-// Before a warp writes its staging area: its last TMA stores have read it.
-__device__ __forceinline__ void staging_free() {
-    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    __syncwarp();
-}
-
-// Sends a warp's staged lines (32 rows x 128 bytes, 16-byte chunks XORed with row % 8, the
-// 128-byte swizzle) to rows r_first + [0, box_rows) and columns n_first on. `whole`: the box may
-// be stored as it is; else only rows below `rows` are, by plain stores.
+// A warp's staged line (32 rows x 128 bytes, 16-byte chunks XORed with row % 8) to the first
+// `count` rows from r_first on, columns n_first on: 8 lanes write a row's 128 bytes. Stores from
+// the registers (32 bytes a lane, each in a row of its own) took 3500 cycles a tile, TMA stores
+// 1000 of issue per warp, this 400.
 template <int size>
-__device__ __forceinline__ void send_lines(const TcArgs& t, const CUtensorMap* tmo, uint8_t* so,
-                                           int lines, int r_first, int64_t rows, int n_first,
-                                           bool whole) {
-    const Fp8Args& a = t.f;
-    constexpr int per = 128 / size;  // columns of a line
-    const int lane = threadIdx.x & 31;
-    if (t.out_tma && whole) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-            for (int l = 0; l < lines; ++l)
-                if (n_first + l * per < a.N)
-                    tma_store_2d(tmo, (n_first + l * per) * size, r_first, so + l * 4096);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
-        return;
-    }
+__device__ __forceinline__ void send_line(const Fp8Args& a, bool aligned, const uint8_t* so,
+                                          int64_t r_first, int count, int n_first) {
+    constexpr int per = 16 / size;
+    const int lane = threadIdx.x & 31, r = lane >> 3;
+    const int n = n_first + (lane & 7) * per;
+    uint8_t* p = static_cast<uint8_t*>(a.out) + ((r_first + r) * a.N + n) * size;
     __syncwarp();
+    if (aligned) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = *reinterpret_cast<const uint4*>(so + (4 * i + r) * 128 +
+                                                   (((lane & 7) ^ ((4 * i + r) & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (4 * i + r < count && n < a.N) *reinterpret_cast<uint4*>(p + 4 * i * a.N * size) = v[i];
+    } else {
 #pragma unroll 1
-    for (int i = 0; i < lines * 8; ++i) {
-        const int rr = (i & 7) * 4 + (lane >> 3), line = i >> 3;
-        const uint4 v = *reinterpret_cast<const uint4*>(so + line * 4096 + rr * 128 +
-                                                        (((lane & 7) ^ (rr & 7)) << 4));
-        const int64_t r = (int64_t)r_first + rr;
-        const int n = n_first + line * per + (lane & 7) * (per / 8);
-        if (rr >= min(t.tile_rows, 32) || r >= rows || n >= a.N) continue;
-        uint8_t* p = static_cast<uint8_t*>(a.out) + (r * a.N + n) * size;
-        if (t.out_tma) {  // 16-byte aligned rows
-            *reinterpret_cast<uint4*>(p) = v;
-        } else {
+        for (int rr = r; rr < count; rr += 4, p += 4 * a.N * size) {
+            const uint4 v = *reinterpret_cast<const uint4*>(so + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
             const uint16_t* h = reinterpret_cast<const uint16_t*>(&v);
-            const int left = (int)min((int64_t)(per / 8), a.N - n) * size / 2;
+            const int left = (int)min((int64_t)per, a.N - n) * size / 2;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (k < left) reinterpret_cast<uint16_t*>(p)[k] = h[k];
         }
     }
+    __syncwarp();
 }
 
 // Out: the output's type; void selects the SiLU form.
 template <int BN, int TR, typename Out, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
-              const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmo) {
+              const __grid_constant__ CUtensorMap tmw) {
     using C = Cfg<BN, TR>;
     constexpr bool SILU = std::is_void<Out>::value;
     extern __shared__ uint8_t smem_raw[];
@@ -365,7 +352,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     uint32_t issued = 0;
     Walk cur = first;
     if (warp < kFoldWarp0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         Ring<C::kStages> st;
         Ring<C::kAcc> tb;
         do {
@@ -384,7 +371,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             src[i] = (int)max((int64_t)0, source_row(a, r0 + 4 * lane + i, rows, e));
-                    const int w_row = (int)(e * a.N) + w.nt * n_step;
+                    const int w_row = w.nt * n_step, w_slab = SILU ? 2 * e : e;
                     for (int g = g_lo; g < g_hi; ++g) {
                         uint8_t* xa = sm.ring[st.idx];
                         uint64_t* fb = &sm.full[st.idx];
@@ -392,10 +379,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
                             mbar_expect_tx(fb, stage_bytes);
                             uint8_t* wb = xa + C::kABytes;
-                            tma_load_2d(wb, &tmw, g * 128, w_row, fb);
-                            if (BN == 256)
-                                tma_load_2d(wb + 128 * 128, &tmw, g * 128,
-                                            SILU ? w_row + (int)(a.N / 2) : w_row + 128, fb);
+                            tma_load_3d(wb, &tmw, g * 128, w_row, w_slab, fb);
                             if (!a.sorted_ids) tma_load_2d(xa, &tmx, g * 128, r0, fb);
                         }
                         __syncwarp();
@@ -491,6 +475,9 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             sm.src[row_of(lane + 32 * i)] =
                                 slot[i] >= 0 && slot[i] < a.num_slots ? slot[i] / a.top_k : -1;
                         __syncwarp();
+                        int src[kRowsPer];
+#pragma unroll
+                        for (int i = 0; i < kRowsPer; ++i) src[i] = sm.src[row0 + i * 4 * kGatherWarps];
                         w.next();
                         if (!SPLIT) look(w);
                         if (!present) {
@@ -506,9 +493,8 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                                 const int tr = row0 + i * 4 * kGatherWarps;
                                 if (tr >= t.tile_rows) break;
                                 // absent rows and columns past K are written as zeros (source size 0)
-                                const int src = sm.src[tr];
-                                const bool ok = src >= 0 && k < a.K;
-                                const uint8_t* p = a.x + (ok ? (int64_t)src * a.K + k : 0);
+                                const bool ok = src[i] >= 0 && k < a.K;
+                                const uint8_t* p = a.x + (ok ? (int64_t)src[i] * a.K + k : 0);
                                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                                                  xa + tr * 128 + ((chunk ^ (tr & 7)) << 4)),
                                              "l"(p), "r"(ok ? 16 : 0)
@@ -536,7 +522,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             }
         } while (SPLIT && cur.more());
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         Ring<C::kAcc> tb;
         do {
             // ---------------- fold + epilogue ----------------
@@ -662,44 +648,38 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             }
                         }
                     } else {
-                        uint8_t* so = sm.stage_out[TR == 32 ? half : fw][0];
-                        const int r_box = (int)r0 + q * 32;
-                        const bool whole = !a.ntp || r_box + min(t.tile_rows, 32) <= rows;
-                        constexpr int kPass = C::kLines * 128 / sizeof(Out);  // columns per pass
-                        constexpr int kPer = 16 / sizeof(Out);
+                        uint8_t* so = sm.stage_out[TR == 32 ? half : fw];
+                        const int64_t r_box = r0 + q * 32;
+                        const int count = (int)min(rows - r_box, (int64_t)min(t.tile_rows - q * 32, 32));
+                        constexpr int kPer = 16 / sizeof(Out), kLine = 8 * kPer;  // columns
 #pragma unroll
-                        for (int c0 = 0; c0 < C::kCols; c0 += kPass) {
-                            staging_free();
+                        for (int c0 = 0; c0 < C::kCols; c0 += kLine) {
 #pragma unroll
-                            for (int c = 0; c < kPass; c += kPer) {
-                                uint32_t u[4];
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    if constexpr (sizeof(Out) == 4) u[i] = __float_as_uint(tot[c0 + c + i]);
-                                    else u[i] = pack2<Out>(tot[c0 + c + 2 * i], tot[c0 + c + 2 * i + 1]);
-                                }
-                                const int chunk = c / kPer;
-                                *reinterpret_cast<uint4*>(so + (chunk / 8) * 4096 + lane * 128 +
-                                                          (((chunk % 8) ^ (lane & 7)) << 4)) =
-                                    make_uint4(u[0], u[1], u[2], u[3]);
+                            for (int i = 0; i < 8; ++i) {
+                                uint4 u;
+                                const float* v = tot + c0 + i * kPer;
+                                if constexpr (sizeof(Out) == 4)
+                                    u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                                   __float_as_uint(v[2]), __float_as_uint(v[3]));
+                                else
+                                    u = make_uint4(pack2<Out>(v[0], v[1]), pack2<Out>(v[2], v[3]),
+                                                   pack2<Out>(v[4], v[5]), pack2<Out>(v[6], v[7]));
+                                *reinterpret_cast<uint4*>(so + lane * 128 + ((i ^ (lane & 7)) << 4)) = u;
                             }
                             if (refill) {
                                 uint32_t v;
                                 if constexpr (sizeof(Out) == 4) v = __float_as_uint(fill);
                                 else v = pack2<Out>(fill, fill);
 #pragma unroll 1
-                                for (int i = 0; i < C::kLines * 8; ++i)
-                                    *reinterpret_cast<uint4*>(so + (i >> 3) * 4096 + lane * 128 + (i & 7) * 16) =
-                                        make_uint4(v, v, v, v);
+                                for (int i = 0; i < 8; ++i)
+                                    *reinterpret_cast<uint4*>(so + lane * 128 + i * 16) = make_uint4(v, v, v, v);
                             }
-                            send_lines<sizeof(Out)>(t, &tmo, so, C::kLines, r_box, rows,
-                                                    (int)n0 + col(c0), whole);
+                            send_line<sizeof(Out)>(a, t.out_vec, so, r_box, count, (int)n0 + col(c0));
                         }
                     }
                     ++done;
                     if (SPLIT) break;
                 }
-                if (!SPLIT && !SILU && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
             __syncwarp();
             if (SPLIT) {
@@ -707,7 +687,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             // CTA `rank` finishes rows rank, rank + S, ... of the cluster's tile
             if (cur.more()) {
                 const int64_t r0 = (int64_t)cur.rb * t.tile_rows, n0 = (int64_t)cur.nt * n_step;
-                const bool vec = t.out_tma;
+                const bool vec = t.out_vec;
                 const float* part = reinterpret_cast<const float*>(sm.ring);
                 for (int tr = rank + S * (warp - kFoldWarp0); tr < t.tile_rows; tr += S * kFoldWarps) {
                     const int64_t r = r0 + tr;
@@ -802,18 +782,16 @@ int sm_count() {
 template <int BN, int TR, typename Out, bool SPLIT>
 int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
     const Fp8Args& a = t.f;
-    CUtensorMap tmx, tmw, tmo{};
-    const int64_t pitch = a.N * (a.out_dtype == 0 ? 4 : 2);
-    t.out_tma = !a.silu && pitch % 16 == 0 && pitch <= INT32_MAX &&
-                (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-    if (t.out_tma && !SPLIT &&
-        !make_tma_map_u8(&tmo, a.out, (uint64_t)a.P, (uint64_t)pitch, 128, std::min(t.tile_rows, 32),
-                         CU_TENSOR_MAP_SWIZZLE_128B))
-        return set_error("fp8_block: tensor map encoding failed");
+    CUtensorMap tmx, tmw;
+    const uintptr_t start = reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.N * (a.out_dtype == 0 ? 4 : 2));
+    t.out_vec = start % 16 == 0;
+    // weight rows as (slab, row, byte): a slab is one expert's matrix, or its gate or up half, so
+    // that one copy brings a tile's gate and up rows
+    const int64_t slab = a.silu ? a.N / 2 : a.N;
     if (!make_tma_map_u8(&tmx, a.x, (uint64_t)a.x_rows, (uint64_t)a.K, 128,
                          a.sorted_ids ? 1 : t.tile_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !make_tma_map_u8(&tmw, a.w, (uint64_t)(a.E * a.N), (uint64_t)a.K, 128, 128,
-                         CU_TENSOR_MAP_SWIZZLE_128B))
+        !make_tma_map_u8_3d(&tmw, a.w, (uint64_t)(a.E * a.N / slab), (uint64_t)slab, (uint64_t)a.K, 128,
+                            a.silu ? 128 : BN, a.silu ? 2 : 1, CU_TENSOR_MAP_SWIZZLE_128B))
         return set_error("fp8_block: tensor map encoding failed");
     auto kern = fp8_tc_kernel<BN, TR, Out, SPLIT>;
     const int smem = (int)sizeof(Smem<BN, TR>) + 1024;
@@ -829,7 +807,7 @@ int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
     at[0].val.clusterDim = {(unsigned)t.split, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = SPLIT ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, t, tmx, tmw, tmo);
+    e = cudaLaunchKernelEx(&cfg, kern, t, tmx, tmw);
     if (e != cudaSuccess) return (int)e;
     return launch_status();
 }

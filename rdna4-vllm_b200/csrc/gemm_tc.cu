@@ -678,6 +678,20 @@ bool make_tma_map_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t
     return make_map(map, base, rows, row_bytes, box_bytes, box_rows, sw);
 }
 
+bool make_tma_map_u8_3d(CUtensorMap* map, const void* base, uint64_t slabs, uint64_t rows,
+                        uint64_t row_bytes, uint32_t box_bytes, uint32_t box_rows,
+                        uint32_t box_slabs, CUtensorMapSwizzle sw) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {row_bytes, rows, slabs};
+    const cuuint64_t strides[2] = {row_bytes, row_bytes * rows};
+    const cuuint32_t box[3] = {box_bytes, box_rows, box_slabs};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box,
+              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool tc_path_ok(int64_t K, int group_size, int e2m1, const void* w, int block_m) {
     return !e2m1 && group_size == 128 && K % 256 == 0 && K >= 256 &&
            (reinterpret_cast<uintptr_t>(w) & 15) == 0 && block_m % 64 == 0;

@@ -97,5 +97,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // (host side; defined in gemm_tc.cu).
 bool make_tma_map_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_bytes,
                      uint32_t box_bytes, uint32_t box_rows, CUtensorMapSwizzle sw);
+// The same with slabs of `rows` rows one after another, box box_bytes x box_rows x box_slabs.
+bool make_tma_map_u8_3d(CUtensorMap* map, const void* base, uint64_t slabs, uint64_t rows,
+                        uint64_t row_bytes, uint32_t box_bytes, uint32_t box_rows,
+                        uint32_t box_slabs, CUtensorMapSwizzle sw);
 
 }  // namespace w4a8
