@@ -26,7 +26,7 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["act_quant.cu", "moe_align.cu", "gemm_mma.cu", "gemv_stream.cu", "gemm_tc.cu", "reduce.cu", "moe_layer.cu", "moe_decode.cu", "ep_dispatch.cu",
               "router.cu", "quant_block.cu", "gemm_fp8_block.cu",
-              "gemm_fp8_tc.cu", "capi.cu"]
+              "gemm_fp8_tc.cu", "gemm_fp8_swap.cu", "capi.cu"]
 LIB = os.path.join(PKG, "libw4a8_b200.so")
 SHIM = os.path.join(PKG, "_C.so")
 

@@ -26,5 +26,6 @@ struct Fp8Args {
 int launch_fp8_simple(const Fp8Args& a, cudaStream_t st);
 bool fp8_tc_ok(const Fp8Args& a);  // sizes and alignment that the tensor-core kernel takes
 int launch_fp8_tc(const Fp8Args& a, cudaStream_t st);
+int launch_fp8_swap(const Fp8Args& a, cudaStream_t st);  // its form for blocks of up to 64 rows
 
 }  // namespace w4a8

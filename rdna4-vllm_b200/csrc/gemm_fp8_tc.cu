@@ -1,21 +1,18 @@
 // gemm_fp8_tc.cu — block-scaled FP8 products on the 5th-generation tensor cores.
 //
-// A tile is up to 128 activation rows (the MMA's M side: row = tensor-memory lane) times BN weight
-// rows (its N side). Per 128-wide block g of K the tensor core returns acc = x_g w_g^T, and the
+// The kernel for blocks of more than 64 rows (fewer: gemm_fp8_swap.cu). A tile is 128 activation
+// rows (the MMA's M side: row = tensor-memory lane) times BN weight rows (its N side). Per 128-wide block g of K the tensor core returns acc = x_g w_g^T, and the
 // fold adds it to fp32 registers with one scalar per thread,
 //     tot[n] += (xs[row, g] * ws[n / 128, g]) * acc[n],
 // because a thread owns one row and the columns of one weight-scale block (two for the SiLU form,
-// gate and up). Tokens sit on the M side even when there are few: the weight rows, which are what
-// has to be read, still pass at the MMA's full N rate, and rows that do not exist are not loaded,
-// folded or stored.
+// gate and up).
 //
 // One persistent CTA per SM, 12 warps:
-//   warp 0     TMA producer: per stage one 128-byte column slab of the tile's x rows (a 2D box, or
-//              tile::gather4 through the routing, one 4-row gather per lane) and BN weight rows,
-//              in the 128-byte swizzle that the MMA's K-major descriptors read.
+//   warp 0     TMA producer: per stage one 128-byte column slab of the tile's x rows and of BN
+//              weight rows, in the 128-byte swizzle that the MMA's K-major descriptors read.
 //   warp 1     owns tensor memory; one thread issues 4 x tcgen05.mma.kind::f8f6f4 (K = 32) per
 //              block into a ring of fp32 accumulators (512 / BN of them).
-//   warps 2, 3 copy the x rows of tall routed tiles (64 or 128 rows) with cp.async instead.
+//   warps 2, 3 copy the x rows of routed tiles with cp.async instead.
 //   warps 4-11 fold: lane quarter warp % 4, one half of the columns each; then the epilogue. They
 //              take the registers that the first four warps give back (setmaxnreg; 128 x 72 +
 //              256 x 216 = 384 x 168, what the block was launched with).
@@ -32,137 +29,44 @@
 // Every mbarrier wait is bounded (sm100.cuh). When one gives up, the CTA stops waiting, waits
 // (boundedly) for its own copies in flight, writes NaN to the tile's outputs and frees tensor
 // memory.
-#include <cuda_bf16.h>
-#include <cudaTypedefs.h>
-
-#include <algorithm>
-#include <type_traits>
-
-#include "common.cuh"
-#include "fp8_block.h"
-#include "internal.h"
-#include "sm100.cuh"
-#include "tcgen05.cuh"
+#include "fp8_tc.cuh"
 
 namespace w4a8 {
 
+using namespace fp8tc;
+
 namespace {
 
-constexpr int kBlk = 128;
-constexpr int kThreads = 384;
 constexpr int kGatherWarps = 2;  // warps 2 and 3
-constexpr int kFoldWarp0 = 4;    // warps 4 to 11 fold
-constexpr int kFoldWarps = 8;
-constexpr int kMaxSplit = 8;
 
-// TR: rows a tile may have, 32 or 128. A short tile's stages hold only its rows; the MMA's
-// 128-row operand then runs on into the weight rows behind them, and those lanes are ignored.
-template <int BN, int TR>
+constexpr int kRows = 128;  // rows of a tile
+
+template <int BN>
 struct Cfg {
-    static constexpr uint32_t kABytes = TR * 128;  // a stage's x slab
+    static constexpr uint32_t kABytes = kRows * 128;  // a stage's x slab
     static constexpr uint32_t kBBytes = BN * 128;
-    static constexpr int kStages = TR == 32 ? (BN == 256 ? 5 : 10) : (BN == 256 ? 4 : 6);
+    static constexpr int kStages = BN == 256 ? 4 : 6;
     static constexpr int kAcc = 512 / BN;
-    static constexpr int kCols = BN / 2;           // columns per fold thread
-    static constexpr int kLive = TR == 32 ? 2 : kFoldWarps;  // fold warps that may hold rows
-    static constexpr int kPitch = BN + 4;          // floats per row of a parked partial tile
+    static constexpr int kCols = BN / 2;   // columns per fold thread
+    static constexpr int kPitch = BN + 4;  // floats per row of a parked partial tile
 };
 
-template <int BN, int TR>
+template <int BN>
 struct Smem {
-    using C = Cfg<BN, TR>;
+    using C = Cfg<BN>;
     uint8_t ring[C::kStages][C::kABytes + C::kBBytes];  // 1024-byte aligned
     // per warp: 32 rows x 128 bytes of finished outputs; the SiLU form keeps the row maxima of its
     // two column halves here, [tile parity][half][row]
-    uint8_t stage_out[C::kLive][4096];
+    uint8_t stage_out[kFoldWarps][4096];
     uint64_t full[C::kStages], empty[C::kStages];
     uint64_t tfull[C::kAcc], tempty[C::kAcc];
-    int src[TR];  // x's rows of the gather warps' tile, -1 for none
+    int src[kRows];  // x's rows of the gather warps' tile, -1 for none
     uint32_t tmem_base;
     int bad;
-    static_assert(C::kABytes + C::kBBytes >= 128 * 128, "the x operand's reads stay in the ring");
-    static_assert(TR * C::kPitch * 4 <= sizeof(ring), "a partial tile fits the ring");
+    static_assert(kRows * C::kPitch * 4 <= sizeof(ring), "a partial tile fits the ring");
 };
-static_assert(sizeof(Smem<256, 128>) + 1024 <= 227 * 1024, "shared memory");
-static_assert(sizeof(Smem<128, 128>) + 1024 <= 227 * 1024, "shared memory");
-static_assert(sizeof(Smem<256, 32>) + 1024 <= 227 * 1024, "shared memory");
-static_assert(sizeof(Smem<128, 32>) + 1024 <= 227 * 1024, "shared memory");
-
-struct TcArgs {
-    Fp8Args f;
-    int tile_rows;  // 16, 32, 64 or 128 rows of x per tile
-    int split;      // CTAs per cluster
-    int n_tiles;    // weight tiles per row block
-    int out_vec;    // out's rows are 16-byte aligned
-};
-
-template <int N>
-struct Ring {
-    uint32_t idx = 0, phase = 0;
-    __device__ __forceinline__ void next() {
-        if (++idx == N) {
-            idx = 0;
-            phase ^= 1;
-        }
-    }
-};
-
-// Tiles of one cluster: t = unit + i * units, t = row_block * n_tiles + n_tile.
-struct Walk {
-    int rb, nt, drb, dnt, n_tiles, blocks;
-    __device__ __forceinline__ Walk(int unit, int units, int n_tiles_, int blocks_)
-        : rb(unit / n_tiles_), nt(unit % n_tiles_), drb(units / n_tiles_), dnt(units % n_tiles_),
-          n_tiles(n_tiles_), blocks(blocks_) {}
-    __device__ __forceinline__ bool more() const { return rb < blocks; }
-    __device__ __forceinline__ void next() {
-        rb += drb;
-        nt += dnt;
-        if (nt >= n_tiles) {
-            nt -= n_tiles;
-            ++rb;
-        }
-    }
-};
-
-// x's row of output row r, or -1 when r is a row of zeros (absent expert e, padding slot).
-__device__ __forceinline__ int64_t source_row(const Fp8Args& a, int64_t r, int64_t rows, int e) {
-    if (r >= rows || e < 0 || e >= a.E) return -1;
-    if (!a.sorted_ids) return r;
-    const int slot = a.sorted_ids[r];
-    return slot >= 0 && slot < a.num_slots ? slot / a.top_k : -1;
-}
-
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
-                                            uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x,
-                                            const int (&y)[4], uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
-        "r"(smem_u32(bar))
-        : "memory");
-}
-
-// Whether a phase is complete, without waiting.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
+static_assert(sizeof(Smem<256>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(sizeof(Smem<128>) + 1024 <= 227 * 1024, "shared memory");
 
 // Waits for the loads into v; the operands keep every use of v behind the wait.
 __device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
@@ -198,59 +102,6 @@ __device__ __forceinline__ void fold_block(uint32_t base, Col col, float f0, flo
         }
         if (j + 16 < kCols) tmem_wait16(next);
     }
-}
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 ld_cluster(const float* p, uint32_t rank) {
-    uint32_t addr;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-
-// silu(g) * u of two outputs, g0 and u0 replaced by the results. One reciprocal serves both
-// denominators d = 1 + exp(-g), 1 / d0 = d1 / (d0 d1): the special-function unit, at 16 a cycle
-// and SM, is what this step waits for. exp(-g) is cut at 2^62 to keep the product in range (silu
-// is below 2^-56 there). Together within 12 units of 2^-24, plus |g| 2^-24 from the exponential's
-// argument: below the product sums' own error.
-__device__ __forceinline__ void silu_mul2(float& g0, float& g1, float u0, float u1) {
-    const float d0 = 1.f + fminf(__expf(-g0), 0x1p62f), d1 = 1.f + fminf(__expf(-g1), 0x1p62f);
-    const float r = __fdividef(1.f, d0 * d1);
-    g0 = g0 * u0 * (d1 * r);
-    g1 = g1 * u1 * (d0 * r);
-}
-
-// Four e4m3 bytes of v / scale, rcp = 1 / scale. The values carry more than the 2^-23 by which the
-// product may miss the quotient; the exact quotient's slow path, 32 times inlined, cost 5x the
-// whole epilogue in instruction fetches.
-__device__ __forceinline__ uint32_t quant4(float v0, float v1, float v2, float v3, float rcp) {
-    return (uint32_t)f32x2_to_e4m3x2(v0 * rcp, v1 * rcp) |
-           (uint32_t)f32x2_to_e4m3x2(v2 * rcp, v3 * rcp) << 16;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // 32 bytes of one row.
@@ -296,14 +147,14 @@ __device__ __forceinline__ void send_line(const Fp8Args& a, bool aligned, const 
 }
 
 // Out: the output's type; void selects the SiLU form.
-template <int BN, int TR, typename Out, bool SPLIT>
+template <int BN, typename Out, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
               const __grid_constant__ CUtensorMap tmw) {
-    using C = Cfg<BN, TR>;
+    using C = Cfg<BN>;
     constexpr bool SILU = std::is_void<Out>::value;
     extern __shared__ uint8_t smem_raw[];
-    Smem<BN, TR>& sm = *reinterpret_cast<Smem<BN, TR>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    Smem<BN>& sm = *reinterpret_cast<Smem<BN>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const Fp8Args& a = t.f;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* bad = &sm.bad;
@@ -311,16 +162,14 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     const int S = SPLIT ? t.split : 1;
     const int rank = SPLIT ? (int)cluster_rank() : 0;
     const int64_t rows = a.ntp ? max((int64_t)0, min((int64_t)a.ntp[0], a.P)) : a.P;
-    const int blocks = (int)((rows + t.tile_rows - 1) / t.tile_rows);
-    const int per_expert = a.expert_ids ? a.block_m / t.tile_rows : 1;
+    const int blocks = (int)((rows + kRows - 1) / kRows);
+    const int per_expert = a.expert_ids ? a.block_m / kRows : 1;
     const int G = (int)a.G;
     const int g_lo = (int)((int64_t)G * rank / S), g_hi = (int)((int64_t)G * (rank + 1) / S);
-    const int live_warps = 2 * ((t.tile_rows + 31) / 32);  // fold warps whose lanes hold rows
     const int n_step = SILU ? 128 : BN;                    // outputs per tile
-    // rows in routing order: short tiles by gather4 (72 cycles of issue per 4 rows), tall ones by
-    // the gather warps' copies (128 rows of gather4 took 2300 cycles a stage, the MMAs 600)
-    const bool copy_rows = TR == 128 && a.sorted_ids != nullptr;
-    const bool tma_gather = TR == 32 && a.sorted_ids != nullptr;
+    // rows in routing order come by the gather warps' copies (128 rows of tile::gather4 took 2300
+    // cycles of issue a stage, three times the MMAs)
+    const bool copy_rows = a.sorted_ids != nullptr;
     const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
     auto expert_of = [&](int rb) { return a.expert_ids ? a.expert_ids[rb / per_expert] : 0; };
 
@@ -332,7 +181,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         }
         for (int s = 0; s < C::kAcc; ++s) {
             mbar_init(&sm.tfull[s], 1);
-            mbar_init(&sm.tempty[s], live_warps);
+            mbar_init(&sm.tempty[s], kFoldWarps);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -358,19 +207,14 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         do {
             if (warp == 0) {
                 // ---------------- TMA producer ----------------
-                const uint32_t stage_bytes = (copy_rows ? 0u : (uint32_t)t.tile_rows * 128) + C::kBBytes;
+                const uint32_t stage_bytes = (copy_rows ? 0u : (uint32_t)kRows * 128) + C::kBBytes;
                 for (Walk w = cur; w.more(); w.next()) {
                     const int e = expert_of(w.rb);
                     if (e < 0 || e >= a.E) {
                         if (SPLIT) break;
                         continue;
                     }
-                    const int r0 = w.rb * t.tile_rows;
-                    int src[4] = {0, 0, 0, 0};  // gathered rows 4 * lane + i; padding rows read row 0
-                    if (tma_gather && 4 * lane < t.tile_rows)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            src[i] = (int)max((int64_t)0, source_row(a, r0 + 4 * lane + i, rows, e));
+                    const int r0 = w.rb * kRows;
                     const int w_row = w.nt * n_step, w_slab = SILU ? 2 * e : e;
                     for (int g = g_lo; g < g_hi; ++g) {
                         uint8_t* xa = sm.ring[st.idx];
@@ -383,8 +227,6 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             if (!a.sorted_ids) tma_load_2d(xa, &tmx, g * 128, r0, fb);
                         }
                         __syncwarp();
-                        if (tma_gather && 4 * lane < t.tile_rows)
-                            tma_gather4(xa + lane * 512, &tmx, g * 128, src, fb);
                         st.next();
                         ++issued;
                     }
@@ -438,12 +280,12 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     }
                 }
                 __syncwarp();
-            } else if (TR == 128 && copy_rows) {
+            } else if (copy_rows) {
                 // ---------------- gather warps: x rows in routing order, tall tiles ----------------
                 // Lane l copies 16-byte chunk l % 8 of rows (l / 8) + 4 (warp index) + 8 i; a stage is
                 // announced when the next one has been requested, so that two are in flight.
                 if (copy_rows) {
-                    constexpr int kRowsPer = TR / (4 * kGatherWarps);
+                    constexpr int kRowsPer = kRows / (4 * kGatherWarps);
                     const int chunk = lane & 7, row0 = (warp - 2) * 4 + (lane >> 3);
                     int pending = -1;  // stage requested but not announced
                     auto announce = [&](int stage) {
@@ -461,8 +303,8 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const int tr = row_of(lane + 32 * i);
-                            const int64_t r = (int64_t)w.rb * t.tile_rows + tr;
-                            slot[i] = tr < t.tile_rows && r < rows ? a.sorted_ids[r] : -1;
+                            const int64_t r = (int64_t)w.rb * kRows + tr;
+                            slot[i] = r < rows ? a.sorted_ids[r] : -1;
                         }
                     };
                     Walk w = cur;
@@ -491,7 +333,6 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
 #pragma unroll
                             for (int i = 0; i < kRowsPer; ++i) {
                                 const int tr = row0 + i * 4 * kGatherWarps;
-                                if (tr >= t.tile_rows) break;
                                 // absent rows and columns past K are written as zeros (source size 0)
                                 const bool ok = src[i] >= 0 && k < a.K;
                                 const uint8_t* p = a.x + (ok ? (int64_t)src[i] * a.K + k : 0);
@@ -528,7 +369,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             // ---------------- fold + epilogue ----------------
             const int q = warp & 3, fw = warp - kFoldWarp0, half = fw >> 2;
             const int row = q * 32 + lane;
-            if (q * 32 < t.tile_rows) {
+            if (q * 32 < kRows) {
                 // column of tot[j]: the plain form's half is contiguous; the SiLU form's holds 64
                 // gate columns, then the 64 matching up columns
                 auto col = [&](int j) {
@@ -544,9 +385,9 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 int next_e = -1, next_slot = -1;    // of the tile to enter next
                 auto look = [&](const Walk& w) {
                     if (!w.more()) return;
-                    const int64_t r = (int64_t)w.rb * t.tile_rows + row;
+                    const int64_t r = (int64_t)w.rb * kRows + row;
                     next_e = expert_of(w.rb);
-                    next_slot = row >= t.tile_rows || r >= rows ? -1 : a.sorted_ids ? a.sorted_ids[r] : (int)r;
+                    next_slot = row >= kRows || r >= rows ? -1 : a.sorted_ids ? a.sorted_ids[r] : (int)r;
                 };
                 auto enter = [&](const Walk& w) {
                     const int e = next_e;
@@ -570,7 +411,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 look(w);
                 if (w.more()) enter(w);
                 while (w.more()) {
-                    const int64_t r0 = (int64_t)w.rb * t.tile_rows, r = r0 + row;
+                    const int64_t r0 = (int64_t)w.rb * kRows, r = r0 + row;
                     const int64_t n0 = (int64_t)w.nt * n_step;
                     const bool is_dead = dead, is_present = present && g_lo < g_hi;
                     w.next();
@@ -604,7 +445,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     const float fill = *bad ? __int_as_float(0x7fffffff) : 0.f;
                     if (SPLIT) {
                         // park the partial tile; the ring is idle once the last accumulator was read
-                        if (row < t.tile_rows) {
+                        if (row < kRows) {
                             float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
 #pragma unroll
                             for (int j = 0; j < C::kCols; j += 4)
@@ -630,7 +471,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         m = fmaxf(m, amax[(half ^ 1) * 128 + row]);
                         const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
                         const float rcp = __frcp_rn(s);
-                        if (row < t.tile_rows && r < rows) {
+                        if (row < kRows && r < rows) {
                             const int64_t inter = a.N / 2;
                             if (half == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
                             uint8_t* p = a.q + r * inter + n0 + half * 64;
@@ -648,9 +489,9 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             }
                         }
                     } else {
-                        uint8_t* so = sm.stage_out[TR == 32 ? half : fw];
+                        uint8_t* so = sm.stage_out[fw];
                         const int64_t r_box = r0 + q * 32;
-                        const int count = (int)min(rows - r_box, (int64_t)min(t.tile_rows - q * 32, 32));
+                        const int count = (int)min(rows - r_box, (int64_t)min(kRows - q * 32, 32));
                         constexpr int kPer = 16 / sizeof(Out), kLine = 8 * kPer;  // columns
 #pragma unroll
                         for (int c0 = 0; c0 < C::kCols; c0 += kLine) {
@@ -684,71 +525,14 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             __syncwarp();
             if (SPLIT) {
                 cluster_sync();
-            // CTA `rank` finishes rows rank, rank + S, ... of the cluster's tile
-            if (cur.more()) {
-                const int64_t r0 = (int64_t)cur.rb * t.tile_rows, n0 = (int64_t)cur.nt * n_step;
-                const bool vec = t.out_vec;
-                const float* part = reinterpret_cast<const float*>(sm.ring);
-                for (int tr = rank + S * (warp - kFoldWarp0); tr < t.tile_rows; tr += S * kFoldWarps) {
-                    const int64_t r = r0 + tr;
-                    if (r >= rows) break;
-                    float4 sum[BN / 128];
-#pragma unroll
-                    for (int c = 0; c < BN / 128; ++c) {
-                        float4 v[kMaxSplit];
-#pragma unroll
-                        for (int k = 0; k < kMaxSplit; ++k)
-                            if (k < S) v[k] = ld_cluster(part + tr * C::kPitch + c * 128 + 4 * lane, k);
-                        sum[c] = v[0];
-#pragma unroll
-                        for (int k = 1; k < kMaxSplit; ++k)
-                            if (k < S) {
-                                sum[c].x += v[k].x;
-                                sum[c].y += v[k].y;
-                                sum[c].z += v[k].z;
-                                sum[c].w += v[k].w;
-                            }
-                    }
-                    if constexpr (SILU) {
-                        const float4 g4 = sum[0], u4 = sum[BN / 128 - 1];
-                        float h[4] = {g4.x, g4.y, g4.z, g4.w};
-                        silu_mul2(h[0], h[1], u4.x, u4.y);
-                        silu_mul2(h[2], h[3], u4.z, u4.w);
-                        float m = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
-                        const float rcp = __frcp_rn(s);
-                        const int64_t inter = a.N / 2;
-                        if (lane == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
-                        *reinterpret_cast<uint32_t*>(a.q + r * inter + n0 + 4 * lane) =
-                            quant4(h[0], h[1], h[2], h[3], rcp);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < BN / 128; ++c) {
-                            const int64_t n = n0 + c * 128 + 4 * lane;
-                            const float o[4] = {sum[c].x, sum[c].y, sum[c].z, sum[c].w};
-                            if constexpr (sizeof(Out) == 4) {
-                                float* p = static_cast<float*>(a.out) + r * a.N + n;
-                                if (vec && n + 4 <= a.N) *reinterpret_cast<float4*>(p) = sum[c];
-                                else
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        if (n + i < a.N) p[i] = o[i];
-                            } else {
-                                uint16_t* p = static_cast<uint16_t*>(a.out) + r * a.N + n;
-                                const uint32_t lo = pack2<Out>(o[0], o[1]);
-                                const uint32_t hi = pack2<Out>(o[2], o[3]);
-                                if (vec && n + 4 <= a.N) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
-                                else
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        if (n + i < a.N) p[i] = (uint16_t)((i < 2 ? lo : hi) >> ((i & 1) * 16));
-                            }
-                        }
-                    }
+                // CTA `rank` finishes rows rank, rank + S, ... of the cluster's tile
+                if (cur.more()) {
+                    const int64_t r0 = (int64_t)cur.rb * kRows, n0 = (int64_t)cur.nt * n_step;
+                    const float* part = reinterpret_cast<const float*>(sm.ring);
+                    for (int tr = rank + S * (warp - kFoldWarp0); tr < kRows && r0 + tr < rows;
+                         tr += S * kFoldWarps)
+                        finish_row<BN, Out>(a, t.out_vec, part + tr * C::kPitch, S, r0 + tr, n0, false);
                 }
-            }
                 // no CTA leaves, or loads its next tile over the parked one, while that is read
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 cluster_sync();
@@ -772,63 +556,23 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     }
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n > 0 ? n : 148;
-}
-
-template <int BN, int TR, typename Out, bool SPLIT>
-int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
-    const Fp8Args& a = t.f;
+template <int BN, typename Out, bool SPLIT>
+int launch_t(const TcArgs& t, int64_t tiles, cudaStream_t st) {
     CUtensorMap tmx, tmw;
-    const uintptr_t start = reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.N * (a.out_dtype == 0 ? 4 : 2));
-    t.out_vec = start % 16 == 0;
-    // weight rows as (slab, row, byte): a slab is one expert's matrix, or its gate or up half, so
-    // that one copy brings a tile's gate and up rows
-    const int64_t slab = a.silu ? a.N / 2 : a.N;
-    if (!make_tma_map_u8(&tmx, a.x, (uint64_t)a.x_rows, (uint64_t)a.K, 128,
-                         a.sorted_ids ? 1 : t.tile_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !make_tma_map_u8_3d(&tmw, a.w, (uint64_t)(a.E * a.N / slab), (uint64_t)slab, (uint64_t)a.K, 128,
-                            a.silu ? 128 : BN, a.silu ? 2 : 1, CU_TENSOR_MAP_SWIZZLE_128B))
+    if (!make_maps(t.f, t.f.sorted_ids ? 1 : kRows, BN, &tmx, &tmw))
         return set_error("fp8_block: tensor map encoding failed");
-    auto kern = fp8_tc_kernel<BN, TR, Out, SPLIT>;
-    const int smem = (int)sizeof(Smem<BN, TR>) + 1024;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, std::max(1, sm_count() / t.split)) * t.split));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)t.split, 1, 1};
-    cfg.attrs = at;
-    cfg.numAttrs = SPLIT ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, t, tmx, tmw);
-    if (e != cudaSuccess) return (int)e;
-    return launch_status();
+    return launch_persistent(fp8_tc_kernel<BN, Out, SPLIT>, t, tiles, sizeof(Smem<BN>) + 1024, tmx,
+                             tmw, st);
 }
 
-template <int TR, typename Out>
+template <typename Out>
 int launch_out(const TcArgs& t, bool bn256, int64_t tiles, cudaStream_t st) {
-    if (bn256) return launch_t<256, TR, Out, false>(t, tiles, st);
-    return t.split > 1 ? launch_t<128, TR, Out, true>(t, tiles, st)
-                       : launch_t<128, TR, Out, false>(t, tiles, st);
-}
-
-template <int TR>
-int launch_tr(const TcArgs& t, bool bn256, int64_t tiles, cudaStream_t st) {
-    if (t.f.silu)
-        return t.split > 1 ? launch_t<256, TR, void, true>(t, tiles, st)
-                           : launch_t<256, TR, void, false>(t, tiles, st);
-    switch (t.f.out_dtype) {
-        case 0: return launch_out<TR, float>(t, bn256, tiles, st);
-        case 1: return launch_out<TR, __half>(t, bn256, tiles, st);
-        default: return launch_out<TR, __nv_bfloat16>(t, bn256, tiles, st);
-    }
+    if constexpr (std::is_void<Out>::value)
+        return t.split > 1 ? launch_t<256, Out, true>(t, tiles, st) : launch_t<256, Out, false>(t, tiles, st);
+    else if (bn256)
+        return launch_t<256, Out, false>(t, tiles, st);
+    else
+        return t.split > 1 ? launch_t<128, Out, true>(t, tiles, st) : launch_t<128, Out, false>(t, tiles, st);
 }
 
 }  // namespace
@@ -840,29 +584,30 @@ bool fp8_tc_ok(const Fp8Args& a) {
 }
 
 int launch_fp8_tc(const Fp8Args& a, cudaStream_t st) {
+    // Up to 64 rows a block the tokens go on the MMA's N side, where they cost by their number.
+    const int64_t rows = a.expert_ids ? a.block_m : a.P;
+    if (rows <= 64) return launch_fp8_swap(a, st);
     TcArgs t{};
     t.f = a;
-    const int64_t rows = a.expert_ids ? a.block_m : a.P;
-    t.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    // row blocks that can hold work: with routing, at most one per slot
-    int64_t blocks = (a.P + t.tile_rows - 1) / t.tile_rows;
-    if (a.sorted_ids) blocks = std::min<int64_t>(blocks, (int64_t)a.num_slots * std::max(1, a.block_m / t.tile_rows));
-    const int sms = sm_count();
+    t.tile_rows = kRows;
+    t.out_vec = out_vec(a);
+    // row blocks that can hold work: with routing, at most one per slot and 128 rows of its block
+    int64_t blocks = (a.P + kRows - 1) / kRows;
+    if (a.sorted_ids) blocks = std::min<int64_t>(blocks, (int64_t)a.num_slots * (a.block_m / kRows));
     const int64_t n = a.silu ? a.N / 2 : a.N;
     // Wide tiles once they fill the GPU; below that, narrow tiles and a cluster along K.
     const int64_t wide = blocks * ((n + (a.silu ? 127 : 255)) / (a.silu ? 128 : 256));
     const int64_t narrow = blocks * ((n + 127) / 128);
-    const bool bn256 = a.silu || wide >= sms;
+    const bool bn256 = a.silu || wide >= sm_count();
     const int64_t tiles = bn256 ? wide : narrow;
     t.n_tiles = (int)(tiles / blocks);
-    // A cluster of 8 (4) finds room on 15 (33) places of the 148 SMs at once, not 18 (37), and a
-    // second round costs more than the wider split gains (16 tiles x 32 blocks of K, M = 128:
-    // 16.9 us with 8, see the commit that limits it).
-    t.split = 1;
-    const int room[4] = {sms, sms / 2, sms * 33 / 148, sms * 15 / 148};
-    for (int i = 1; i < 4; ++i)
-        if (tiles <= room[i] && a.G >= (2 << i)) t.split = 1 << i;
-    return t.tile_rows <= 32 ? launch_tr<32>(t, bn256, tiles, st) : launch_tr<128>(t, bn256, tiles, st);
+    t.split = split_for(tiles, a.G);
+    if (a.silu) return launch_out<void>(t, bn256, tiles, st);
+    switch (a.out_dtype) {
+        case 0: return launch_out<float>(t, bn256, tiles, st);
+        case 1: return launch_out<__half>(t, bn256, tiles, st);
+        default: return launch_out<__nv_bfloat16>(t, bn256, tiles, st);
+    }
 }
 
 }  // namespace w4a8
