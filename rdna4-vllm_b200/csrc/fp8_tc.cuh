@@ -261,9 +261,9 @@ inline bool out_vec(const Fp8Args& a) {
 }
 
 // Persistent launch of `tiles` tiles over clusters of t.split CTAs.
-template <typename Kernel>
-int launch_persistent(Kernel kern, const TcArgs& t, int64_t tiles, size_t smem, const CUtensorMap& tmx,
-                      const CUtensorMap& tmw, cudaStream_t st) {
+template <typename Kernel, typename... Maps>
+int launch_persistent(Kernel kern, const TcArgs& t, int64_t tiles, size_t smem, cudaStream_t st,
+                      const Maps&... maps) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg{};
@@ -276,7 +276,7 @@ int launch_persistent(Kernel kern, const TcArgs& t, int64_t tiles, size_t smem, 
     at[0].val.clusterDim = {(unsigned)t.split, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = t.split > 1 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, t, tmx, tmw);
+    e = cudaLaunchKernelEx(&cfg, kern, t, maps...);
     return e != cudaSuccess ? (int)e : launch_status();
 }
 

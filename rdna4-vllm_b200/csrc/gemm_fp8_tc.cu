@@ -37,36 +37,38 @@ using namespace fp8tc;
 
 namespace {
 
-constexpr int kGatherWarps = 2;  // warps 2 and 3
-
 constexpr int kRows = 128;  // rows of a tile
 
-template <int BN>
+// kStaged: outputs leave by TMA from a staging area (not the SiLU form's bytes, nor a split tile).
+template <int BN, bool kStaged>
 struct Cfg {
     static constexpr uint32_t kABytes = kRows * 128;  // a stage's x slab
     static constexpr uint32_t kBBytes = BN * 128;
-    static constexpr int kStages = BN == 256 ? 4 : 6;
+    static constexpr int kStages = BN == 256 ? (kStaged ? 3 : 4) : 6;
     static constexpr int kAcc = 512 / BN;
     static constexpr int kCols = BN / 2;   // columns per fold thread
+    static constexpr int kLines = kCols / 64;  // 128-byte lines that a warp's staging area holds
     static constexpr int kPitch = BN + 4;  // floats per row of a parked partial tile
 };
 
-template <int BN>
+template <int BN, bool kStaged>
 struct Smem {
-    using C = Cfg<BN>;
+    using C = Cfg<BN, kStaged>;
     uint8_t ring[C::kStages][C::kABytes + C::kBBytes];  // 1024-byte aligned
-    // per warp: 32 rows x 128 bytes of finished outputs; the SiLU form keeps the row maxima of its
-    // two column halves here, [tile parity][half][row]
-    uint8_t stage_out[kFoldWarps][4096];
+    // finished outputs: [column half][line][row] x 128 bytes, 16-byte chunks XORed with row % 8
+    uint8_t stage_out[kStaged ? 2 : 0][C::kLines][kRows * 128];
+    float amax[kStaged ? 0 : 2][2][kRows];  // SiLU form: row maxima, [tile parity][column half]
     uint64_t full[C::kStages], empty[C::kStages];
     uint64_t tfull[C::kAcc], tempty[C::kAcc];
+    uint64_t ofull[2 * C::kLines], ofree[2 * C::kLines];  // staged lines
     int src[kRows];  // x's rows of the gather warps' tile, -1 for none
     uint32_t tmem_base;
     int bad;
     static_assert(kRows * C::kPitch * 4 <= sizeof(ring), "a partial tile fits the ring");
 };
-static_assert(sizeof(Smem<256>) + 1024 <= 227 * 1024, "shared memory");
-static_assert(sizeof(Smem<128>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(sizeof(Smem<256, true>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(sizeof(Smem<256, false>) + 1024 <= 227 * 1024, "shared memory");
+static_assert(sizeof(Smem<128, true>) + 1024 <= 227 * 1024, "shared memory");
 
 // Waits for the loads into v; the operands keep every use of v behind the wait.
 __device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
@@ -111,31 +113,28 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&u)[8]) {
                  : "memory");
 }
 
-// A warp's staged line (32 rows x 128 bytes, 16-byte chunks XORed with row % 8) to the first
-// `count` rows from r_first on, columns n_first on: 8 lanes write a row's 128 bytes. Stores from
-// the registers (32 bytes a lane, each in a row of its own) took 3500 cycles a tile, TMA stores
-// 1000 of issue per warp, this 400.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(smem_u32(src))
+                 : "memory");
+}
+
+// A warp's 32 rows of a staged line to the first `count` rows from r_first on, columns n_first on,
+// by plain stores: tiles that TMA cannot store whole, and rows that are not 16-byte aligned.
 template <int size>
-__device__ __forceinline__ void send_line(const Fp8Args& a, bool aligned, const uint8_t* so,
-                                          int64_t r_first, int count, int n_first) {
+__device__ __noinline__ void send_line(const Fp8Args& a, bool aligned, const uint8_t* so,
+                                       int64_t r_first, int count, int n_first) {
     constexpr int per = 16 / size;
     const int lane = threadIdx.x & 31, r = lane >> 3;
     const int n = n_first + (lane & 7) * per;
     uint8_t* p = static_cast<uint8_t*>(a.out) + ((r_first + r) * a.N + n) * size;
-    __syncwarp();
-    if (aligned) {
-        uint4 v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = *reinterpret_cast<const uint4*>(so + (4 * i + r) * 128 +
-                                                   (((lane & 7) ^ ((4 * i + r) & 7)) << 4));
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (4 * i + r < count && n < a.N) *reinterpret_cast<uint4*>(p + 4 * i * a.N * size) = v[i];
-    } else {
-#pragma unroll 1
-        for (int rr = r; rr < count; rr += 4, p += 4 * a.N * size) {
-            const uint4 v = *reinterpret_cast<const uint4*>(so + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+    for (int rr = r; rr < count; rr += 4, p += 4 * a.N * size) {
+        const uint4 v = *reinterpret_cast<const uint4*>(so + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+        if (n >= a.N) continue;
+        if (aligned) {
+            *reinterpret_cast<uint4*>(p) = v;
+        } else {
             const uint16_t* h = reinterpret_cast<const uint16_t*>(&v);
             const int left = (int)min((int64_t)per, a.N - n) * size / 2;
 #pragma unroll
@@ -143,18 +142,18 @@ __device__ __forceinline__ void send_line(const Fp8Args& a, bool aligned, const 
                 if (k < left) reinterpret_cast<uint16_t*>(p)[k] = h[k];
         }
     }
-    __syncwarp();
 }
 
 // Out: the output's type; void selects the SiLU form.
 template <int BN, typename Out, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
-              const __grid_constant__ CUtensorMap tmw) {
-    using C = Cfg<BN>;
+              const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmo) {
     constexpr bool SILU = std::is_void<Out>::value;
+    constexpr bool kStaged = !SILU && !SPLIT;
+    using C = Cfg<BN, kStaged>;
     extern __shared__ uint8_t smem_raw[];
-    Smem<BN>& sm = *reinterpret_cast<Smem<BN>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    Smem<BN, kStaged>& sm = *reinterpret_cast<Smem<BN, kStaged>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const Fp8Args& a = t.f;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* bad = &sm.bad;
@@ -170,6 +169,12 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     // rows in routing order come by the gather warps' copies (128 rows of tile::gather4 took 2300
     // cycles of issue a stage, three times the MMAs)
     const bool copy_rows = a.sorted_ids != nullptr;
+    constexpr int kGatherWarps = kStaged ? 1 : 2;  // warp 3 then sends the outputs
+    // tiles whose 128 rows TMA may store: the rows past the last one in use are not ours
+    auto tma_out = [&](int rb) { return t.out_vec && (!a.ntp || (int64_t)(rb + 1) * kRows <= rows); };
+    constexpr int kOutSize = SILU ? 1 : sizeof(std::conditional_t<SILU, char, Out>);
+    constexpr int kLineCols = 128 / kOutSize;                      // columns of a staged line
+    constexpr int kRounds = C::kCols / (C::kLines * kLineCols);    // staging areas per tile
     const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
     auto expert_of = [&](int rb) { return a.expert_ids ? a.expert_ids[rb / per_expert] : 0; };
 
@@ -182,6 +187,10 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         for (int s = 0; s < C::kAcc; ++s) {
             mbar_init(&sm.tfull[s], 1);
             mbar_init(&sm.tempty[s], kFoldWarps);
+        }
+        for (int s = 0; s < 2 * C::kLines; ++s) {
+            mbar_init(&sm.ofull[s], 4);  // the four lane quarters
+            mbar_init(&sm.ofree[s], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -280,6 +289,27 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     }
                 }
                 __syncwarp();
+            } else if (kStaged && warp == 3) {
+                // ---------------- output warp: staged lines, 64 x 128 outputs a copy ----------------
+                // (a TMA store costs its thread some 500 cycles; the fold warps have none to spare)
+                if (lane < 2 * C::kLines) {
+                    const int half = lane / C::kLines, line = lane % C::kLines;
+                    int turn = 0;
+                    for (Walk w = cur; w.more(); w.next()) {
+                        if (!tma_out(w.rb)) continue;
+                        for (int i = 0; i < kRounds; ++i, turn ^= 1) {
+                            const int n = w.nt * n_step + half * C::kCols + (i * C::kLines + line) * kLineCols;
+                            mbar_wait(&sm.ofull[lane], turn, bad);
+                            if (n < a.N)
+                                tma_store_2d(&tmo, n * kOutSize, w.rb * kRows, sm.stage_out[half][line]);
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                            mbar_arrive(&sm.ofree[lane]);
+                        }
+                    }
+                    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+                }
+                __syncwarp();
             } else if (copy_rows) {
                 // ---------------- gather warps: x rows in routing order, tall tiles ----------------
                 // Lane l copies 16-byte chunk l % 8 of rows (l / 8) + 4 (warp index) + 8 i; a stage is
@@ -294,14 +324,15 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         if (lane == 0) mbar_arrive(&sm.full[stage]);
                     };
                     // the routing entries of the tile to enter next, fetched a tile ahead: lane l
-                    // holds this warp's rows l and l + 32 (of 64), the rows of warp 2 + (row / 4) % 2
-                    int slot[2] = {-1, -1}, e = -1;
-                    auto row_of = [&](int i) { return (i >> 2) * 8 + (warp - 2) * 4 + (i & 3); };
+                    // holds this warp's rows l, l + 32, ...: row groups of 4 are dealt to the warps
+                    constexpr int kSlots = 4 / kGatherWarps;
+                    int slot[kSlots], e = -1;
+                    auto row_of = [&](int i) { return (i >> 2) * 4 * kGatherWarps + (warp - 2) * 4 + (i & 3); };
                     auto look = [&](const Walk& w) {
                         if (!w.more()) return;
                         e = expert_of(w.rb);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
+                        for (int i = 0; i < kSlots; ++i) {
                             const int tr = row_of(lane + 32 * i);
                             const int64_t r = (int64_t)w.rb * kRows + tr;
                             slot[i] = r < rows ? a.sorted_ids[r] : -1;
@@ -313,13 +344,15 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         const bool present = e >= 0 && e < a.E;
                         __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
+                        for (int i = 0; i < kSlots; ++i)
                             sm.src[row_of(lane + 32 * i)] =
                                 slot[i] >= 0 && slot[i] < a.num_slots ? slot[i] / a.top_k : -1;
                         __syncwarp();
-                        int src[kRowsPer];
+                        int src[kRowsPer <= 16 ? kRowsPer : 1];  // or from shared memory each time
+                        if (kRowsPer <= 16)
 #pragma unroll
-                        for (int i = 0; i < kRowsPer; ++i) src[i] = sm.src[row0 + i * 4 * kGatherWarps];
+                            for (int i = 0; i < kRowsPer; ++i)
+                                src[i % (kRowsPer <= 16 ? kRowsPer : 1)] = sm.src[row0 + i * 4 * kGatherWarps];
                         w.next();
                         if (!SPLIT) look(w);
                         if (!present) {
@@ -334,8 +367,9 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             for (int i = 0; i < kRowsPer; ++i) {
                                 const int tr = row0 + i * 4 * kGatherWarps;
                                 // absent rows and columns past K are written as zeros (source size 0)
-                                const bool ok = src[i] >= 0 && k < a.K;
-                                const uint8_t* p = a.x + (ok ? (int64_t)src[i] * a.K + k : 0);
+                                const int sr = kRowsPer <= 16 ? src[i % (kRowsPer <= 16 ? kRowsPer : 1)] : sm.src[tr];
+                                const bool ok = sr >= 0 && k < a.K;
+                                const uint8_t* p = a.x + (ok ? (int64_t)sr * a.K + k : 0);
                                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                                                  xa + tr * 128 + ((chunk ^ (tr & 7)) << 4)),
                                              "l"(p), "r"(ok ? 16 : 0)
@@ -376,7 +410,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     return SILU ? (j < 64 ? half * 64 + j : 128 + half * 64 + j - 64) : half * C::kCols + j;
                 };
                 const int64_t NB = (a.N + kBlk - 1) / kBlk;
-                int done = 0;
+                int done = 0, turn = 0;  // turn: phase of the staging area
                 // The scales of a tile's first block are fetched while the tile before it folds its
                 // last one, its routing entries a whole tile ahead: neither wait is paid per tile.
                 const float *xs = a.xs, *ws0 = a.ws, *ws1 = a.ws;
@@ -443,7 +477,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     // `fill` over its staged row (a wait that gave up makes every row one, of NaN)
                     const bool refill = is_dead || *bad;
                     const float fill = *bad ? __int_as_float(0x7fffffff) : 0.f;
-                    if (SPLIT) {
+                    if constexpr (SPLIT) {
                         // park the partial tile; the ring is idle once the last accumulator was read
                         if (row < kRows) {
                             float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
@@ -465,10 +499,10 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         }
                         if (refill) m = fill;
                         // the row's other 64 outputs are with the warp of the other half
-                        float* amax = reinterpret_cast<float*>(sm.stage_out) + (done & 1) * 256;
-                        amax[half * 128 + row] = m;
+                        float(&amax)[2][kRows] = sm.amax[done & 1];
+                        amax[half][row] = m;
                         asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
-                        m = fmaxf(m, amax[(half ^ 1) * 128 + row]);
+                        m = fmaxf(m, amax[half ^ 1][row]);
                         const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
                         const float rcp = __frcp_rn(s);
                         if (row < kRows && r < rows) {
@@ -489,33 +523,55 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             }
                         }
                     } else {
-                        uint8_t* so = sm.stage_out[fw];
-                        const int64_t r_box = r0 + q * 32;
-                        const int count = (int)min(rows - r_box, (int64_t)min(kRows - q * 32, 32));
-                        constexpr int kPer = 16 / sizeof(Out), kLine = 8 * kPer;  // columns
+                        const bool by_tma = tma_out((int)(r0 / kRows));
+                        const int64_t r_warp = r0 + q * 32;
+                        const int count = (int)min(rows - r_warp, (int64_t)32);
+                        constexpr int kPer = 16 / sizeof(Out);
 #pragma unroll
-                        for (int c0 = 0; c0 < C::kCols; c0 += kLine) {
+                        for (int i = 0; i < kRounds; ++i) {
+                            uint8_t* so = sm.stage_out[half][0] + q * 4096;
+                            if (by_tma) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                uint4 u;
-                                const float* v = tot + c0 + i * kPer;
-                                if constexpr (sizeof(Out) == 4)
-                                    u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
-                                                   __float_as_uint(v[2]), __float_as_uint(v[3]));
-                                else
-                                    u = make_uint4(pack2<Out>(v[0], v[1]), pack2<Out>(v[2], v[3]),
-                                                   pack2<Out>(v[4], v[5]), pack2<Out>(v[6], v[7]));
-                                *reinterpret_cast<uint4*>(so + lane * 128 + ((i ^ (lane & 7)) << 4)) = u;
+                                for (int l = 0; l < C::kLines; ++l)
+                                    mbar_wait(&sm.ofree[half * C::kLines + l], turn ^ 1, bad);
                             }
+#pragma unroll
+                            for (int l = 0; l < C::kLines; ++l)
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) {
+                                    uint4 u;
+                                    const float* v = tot + (i * C::kLines + l) * kLineCols + c * kPer;
+                                    if constexpr (sizeof(Out) == 4)
+                                        u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                                       __float_as_uint(v[2]), __float_as_uint(v[3]));
+                                    else
+                                        u = make_uint4(pack2<Out>(v[0], v[1]), pack2<Out>(v[2], v[3]),
+                                                       pack2<Out>(v[4], v[5]), pack2<Out>(v[6], v[7]));
+                                    *reinterpret_cast<uint4*>(so + l * (kRows * 128) + lane * 128 +
+                                                              ((c ^ (lane & 7)) << 4)) = u;
+                                }
                             if (refill) {
                                 uint32_t v;
                                 if constexpr (sizeof(Out) == 4) v = __float_as_uint(fill);
                                 else v = pack2<Out>(fill, fill);
 #pragma unroll 1
-                                for (int i = 0; i < 8; ++i)
-                                    *reinterpret_cast<uint4*>(so + lane * 128 + i * 16) = make_uint4(v, v, v, v);
+                                for (int c = 0; c < 8 * C::kLines; ++c)
+                                    *reinterpret_cast<uint4*>(so + (c >> 3) * (kRows * 128) + lane * 128 +
+                                                              (c & 7) * 16) = make_uint4(v, v, v, v);
                             }
-                            send_line<sizeof(Out)>(a, t.out_vec, so, r_box, count, (int)n0 + col(c0));
+                            if (by_tma) {
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                                __syncwarp();
+                                if (lane < C::kLines) mbar_arrive(&sm.ofull[half * C::kLines + lane]);
+                                turn ^= 1;
+                            } else {
+                                __syncwarp();
+                                for (int l = 0; l < C::kLines; ++l)
+                                    send_line<sizeof(Out)>(a, t.out_vec, so + l * (kRows * 128), r_warp, count,
+                                                           (int)n0 + half * C::kCols +
+                                                               (i * C::kLines + l) * kLineCols);
+                                __syncwarp();
+                            }
                         }
                     }
                     ++done;
@@ -557,12 +613,19 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
 }
 
 template <int BN, typename Out, bool SPLIT>
-int launch_t(const TcArgs& t, int64_t tiles, cudaStream_t st) {
-    CUtensorMap tmx, tmw;
-    if (!make_maps(t.f, t.f.sorted_ids ? 1 : kRows, BN, &tmx, &tmw))
+int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
+    constexpr bool kStaged = !std::is_void<Out>::value && !SPLIT;
+    const Fp8Args& a = t.f;
+    CUtensorMap tmx, tmw, tmo{};
+    if (!make_maps(a, a.sorted_ids ? 1 : kRows, BN, &tmx, &tmw))
         return set_error("fp8_block: tensor map encoding failed");
-    return launch_persistent(fp8_tc_kernel<BN, Out, SPLIT>, t, tiles, sizeof(Smem<BN>) + 1024, tmx,
-                             tmw, st);
+    const int64_t pitch = a.N * (a.out_dtype == 0 ? 4 : 2);
+    if (kStaged && pitch > INT32_MAX) t.out_vec = 0;  // beyond a TMA coordinate
+    if (kStaged && t.out_vec &&
+        !make_tma_map_u8(&tmo, a.out, (uint64_t)a.P, (uint64_t)pitch, 128, kRows, CU_TENSOR_MAP_SWIZZLE_128B))
+        return set_error("fp8_block: tensor map encoding failed");
+    return launch_persistent(fp8_tc_kernel<BN, Out, SPLIT>, t, tiles, sizeof(Smem<BN, kStaged>) + 1024,
+                             st, tmx, tmw, tmo);
 }
 
 template <typename Out>
