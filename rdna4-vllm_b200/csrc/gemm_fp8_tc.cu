@@ -12,7 +12,8 @@
 //              weight rows, in the 128-byte swizzle that the MMA's K-major descriptors read.
 //   warp 1     owns tensor memory; one thread issues 4 x tcgen05.mma.kind::f8f6f4 (K = 32) per
 //              block into a ring of fp32 accumulators (512 / BN of them).
-//   warps 2, 3 copy the x rows of routed tiles with cp.async instead.
+//   warps 2, 3 copy the x rows of routed tiles with cp.async instead; warp 3 sends finished 16- and
+//              32-bit outputs by TMA.
 //   warps 4-11 fold: lane quarter warp % 4, one half of the columns each; then the epilogue. They
 //              take the registers that the first four warps give back (setmaxnreg; 128 x 72 +
 //              256 x 216 = 384 x 168, what the block was launched with).
@@ -22,9 +23,11 @@
 // sums rows r, r + S, ... over the cluster in rank order (distributed shared memory), so the
 // result does not depend on timing.
 //
-// What bounds it. A block of a 128 x 256 tile is 512 cycles of MMA at the tensor cores' rate, but
-// the shared memory takes 96 KB of traffic for it (48 KB written by TMA, 48 KB read by the MMA),
-// 768 cycles; measured, a thread that issues one block after another is held up for 770.
+// What bounds it. A block of a 128 x 256 tile is 512 cycles of MMA, but its 48 KB come from L2 at 57
+// to 64 bytes a cycle and SM, 770 to 840 cycles however little is computed on them, and long runs
+// sit at the 1000 W power cap (1.6 to 1.7 GHz). A pair of CTAs on a tile of 256 x 256 (cta_group::2,
+// 32 KB a block) was slower, 197 us against 173 at 8192 x 8192 x 2048: with a fold after every
+// block only two accumulators fit, and the way from MMA to both CTAs' folds and back is 2400 cycles.
 //
 // Every mbarrier wait is bounded (sm100.cuh). When one gives up, the CTA stops waiting, waits
 // (boundedly) for its own copies in flight, writes NaN to the tile's outputs and frees tensor

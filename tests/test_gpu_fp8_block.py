@@ -142,7 +142,8 @@ def test_rms_norm_quant_residual_in_place(w4):
 GEMMS = [(1, 1, 16), (1, 128, 128), (3, 129, 144), (16, 256, 512), (17, 33, 7), (128, 256, 384),
          (129, 257, 1040), (200, 1000, 656), (64, 512, 2048), (1, 4096, 2048), (300, 384, 200),
          (2, 8192, 128), (1000, 640, 1152), (513, 2048, 272), (5, 136, 8192), (33, 2048, 4096),
-         (260, 260, 2064)]
+         (260, 260, 2064), (2500, 2100, 400), (2432, 2048, 256), (1281, 4001, 144),
+         (130, 19000, 256), (100, 38000, 128), (385, 12800, 384)]
 
 
 @pytest.mark.parametrize("dtype", [FP16, BF16, FP32])
