@@ -68,6 +68,19 @@ __device__ __forceinline__ int64_t source_row(const Fp8Args& a, int64_t r, int64
     return slot >= 0 && slot < a.num_slots ? slot / a.top_k : -1;
 }
 
+// True in one lane of a converged warp. The copies, MMAs and commits take uniform operands, and
+// behind this condition the compiler need not serialise the lanes to make them so (a comparison
+// of the lane number cost 200 cycles for each).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
                                             uint64_t* bar) {
     asm volatile(

@@ -99,6 +99,10 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
     auto expert_of = [&](int rb) { return a.expert_ids ? a.expert_ids[rb] : 0; };
 
+    if (tid == 32 * 2) {
+        prefetch_map(&tmx);
+        prefetch_map(&tmw);
+    }
     if (tid == 0) {
         sm.bad = 0;
         for (int s = 0; s < C::kStages; ++s) {
@@ -157,7 +161,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     uint8_t* ws = sm.ring[st.idx];
                     uint8_t* xs = ws + C::kWBytes;
                     uint64_t* fb = &sm.full[st.idx];
-                    if (lane == 0) {
+                    if (elect_one()) {
                         mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
                         mbar_expect_tx(fb, C::kWBytes + C::kXBytes);
                         tma_load_3d(ws, &tmw, g * 128, w_row, w_slab, fb);
@@ -173,7 +177,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             __syncwarp();
         } else if (warp == 1) {
             // ---------------- MMA issuer ----------------
-            if (lane == 0) {
+            if (elect_one()) {
                 constexpr uint32_t idesc = umma_idesc(128, NT);
                 for (Walk w = cur; w.more(); w.next()) {
                     const int e = expert_of(w.rb);

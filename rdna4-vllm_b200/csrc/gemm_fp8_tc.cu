@@ -181,6 +181,10 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
     auto expert_of = [&](int rb) { return a.expert_ids ? a.expert_ids[rb / per_expert] : 0; };
 
+    if (tid == 32 * 2) {
+        prefetch_map(&tmx);
+        prefetch_map(&tmw);
+    }
     if (tid == 0) {
         sm.bad = 0;
         for (int s = 0; s < C::kStages; ++s) {
@@ -231,7 +235,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     for (int g = g_lo; g < g_hi; ++g) {
                         uint8_t* xa = sm.ring[st.idx];
                         uint64_t* fb = &sm.full[st.idx];
-                        if (lane == 0) {
+                        if (elect_one()) {
                             mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
                             mbar_expect_tx(fb, stage_bytes);
                             uint8_t* wb = xa + C::kABytes;
@@ -247,7 +251,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 __syncwarp();
             } else if (warp == 1) {
                 // ---------------- MMA issuer ----------------
-                if (lane == 0) {
+                if (elect_one()) {
                     constexpr uint32_t idesc = umma_idesc(128, BN);
                     bool full = false, room = false;  // the next block's barriers were seen complete
                     for (Walk w = cur; w.more(); w.next()) {
