@@ -118,9 +118,20 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_arrive() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    cluster_arrive();
+    cluster_wait();
+}
+__device__ __forceinline__ void st_cluster(const float* p, uint32_t rank, float v) {
+    uint32_t addr;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ float4 ld_cluster(const float* p, uint32_t rank) {
     uint32_t addr;
@@ -166,34 +177,31 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Sums a parked row over the cluster's S CTAs in rank order and writes its outputs. part: the row's
-// W floats (the SiLU form: 128 gate, then 128 up) at the same place in every CTA's shared memory;
-// n0: the first output. One warp; lane l has columns 4 l of each 128. `dead`: a row of zeros.
-template <int W, typename Out>
-__device__ __forceinline__ void finish_row(const Fp8Args& a, bool vec, const float* part, int S,
+// Adds the S parts of a row, `stride` floats apart in this CTA's shared memory (kRemote: at the same
+// place in each CTA of the cluster), in rank order, and writes its outputs. A part is W floats (the
+// SiLU form: 128 gate, then 128 up); n0: the first output. One warp; lane l has columns 4 l of each
+// 128. `dead`: a row of zeros.
+template <int W, typename Out, bool kRemote>
+__device__ __forceinline__ void finish_row(const Fp8Args& a, bool vec, const float* part, int S, int stride,
                                            int64_t r, int64_t n0, bool dead) {
     const int lane = threadIdx.x & 31;
     float4 sum[W / 128];
 #pragma unroll
     for (int c = 0; c < W / 128; ++c) {
         const float* p = part + c * 128 + 4 * lane;
-        if (S == 1) {
-            sum[c] = *reinterpret_cast<const float4*>(p);
-        } else {
-            float4 v[kMaxSplit];
+        float4 v[kMaxSplit];
 #pragma unroll
-            for (int k = 0; k < kMaxSplit; ++k)
-                if (k < S) v[k] = ld_cluster(p, k);
-            sum[c] = v[0];
+        for (int k = 0; k < kMaxSplit; ++k)
+            if (k < S) v[k] = kRemote ? ld_cluster(p, k) : *reinterpret_cast<const float4*>(p + k * stride);
+        sum[c] = v[0];
 #pragma unroll
-            for (int k = 1; k < kMaxSplit; ++k)
-                if (k < S) {
-                    sum[c].x += v[k].x;
-                    sum[c].y += v[k].y;
-                    sum[c].z += v[k].z;
-                    sum[c].w += v[k].w;
-                }
-        }
+        for (int k = 1; k < kMaxSplit; ++k)
+            if (k < S) {
+                sum[c].x += v[k].x;
+                sum[c].y += v[k].y;
+                sum[c].z += v[k].z;
+                sum[c].w += v[k].w;
+            }
         if (dead) sum[c] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if constexpr (std::is_void<Out>::value) {

@@ -16,7 +16,9 @@
 // One persistent CTA per SM, 12 warps: 0 TMA producer (x rows by a 2D box, or by tile::gather4
 // through the routing, 4 rows a lane), 1 tensor memory and MMA issue, 2 and 3 idle (a lane quarter
 // needs warps 4 k + q), 4-11 fold: lane quarter warp % 4, one half of the tokens each. With few
-// tiles a cluster of S CTAs shares one along K and sums the parked tiles in rank order.
+// tiles a cluster of S CTAs shares one along K: token c belongs to CTA c % S, every CTA parks its
+// part of it there (distributed shared memory), and after a cluster barrier the owner adds the parts
+// in rank order.
 //
 // Waits are bounded as in gemm_fp8_tc.cu: one that gives up leaves NaN in the tile's outputs.
 #include "fp8_tc.cuh"
@@ -103,17 +105,20 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         prefetch_map(&tmx);
         prefetch_map(&tmw);
     }
-    if (tid == 0) {
-        sm.bad = 0;
-        for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(&sm.full[s], 1);
-            mbar_init(&sm.empty[s], 1);
+    // The producer sets up its barriers and goes on to its first copies; the others meet when the
+    // tensor memory is there too.
+    if (warp == 0) {
+        if (lane == 0) sm.bad = 0;
+        if (lane < C::kStages) {
+            mbar_init(&sm.full[lane], 1);
+            mbar_init(&sm.empty[lane], 1);
         }
-        for (int s = 0; s < C::kAcc; ++s) {
-            mbar_init(&sm.tfull[s], 1);
-            mbar_init(&sm.tempty[s], kFoldWarps);
+        if (lane < C::kAcc) {
+            mbar_init(&sm.tfull[lane], 1);
+            mbar_init(&sm.tempty[lane], kFoldWarps);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        __syncwarp();
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -121,10 +126,14 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                      "r"(C::kTmemCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::);
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::);
-    const uint32_t tmem = sm.tmem_base;
+    if (warp == 0) {
+        asm volatile("bar.arrive 8, %0;" ::"n"(kThreads) : "memory");
+    } else {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::);
+        asm volatile("bar.sync 8, %0;" ::"n"(kThreads) : "memory");
+        asm volatile("tcgen05.fence::after_thread_sync;" ::);
+    }
+    if (SPLIT) cluster_arrive();  // awaited before the first part is parked with another CTA
 
     // One pass runs all of the CTA's tiles; with a split it is one tile, and the cluster meets
     // before the next. Each role keeps its ring positions over the passes.
@@ -186,7 +195,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         mbar_wait(&sm.tempty[tb.idx], tb.phase ^ 1, bad);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::);
                         const uint32_t wa = smem_u32(sm.ring[st.idx]);
-                        const uint32_t d = tmem + tb.idx * C::kAccCols;
+                        const uint32_t d = sm.tmem_base + tb.idx * C::kAccCols;
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
                             const uint64_t db = desc_sw128(wa + C::kWBytes + kk * 32);
@@ -283,7 +292,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::);
                         const uint32_t base =
-                            tmem + ((uint32_t)(q * 32) << 16) + tb.idx * C::kAccCols + half * C::kHalf;
+                            sm.tmem_base + ((uint32_t)(q * 32) << 16) + tb.idx * C::kAccCols + half * C::kHalf;
                         uint32_t v[C::kSub][C::kHalf];
 #pragma unroll
                         for (int b = 0; b < C::kSub; ++b) tmem_load(base + b * NT, v[b]);
@@ -310,32 +319,46 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             }
                     }
                 }
-                // park the tile; the rows of the one before are written by now
-                if (!SPLIT) asm volatile("bar.sync 1, %0;" ::"n"(kFoldWarps * 32) : "memory");
-                if (q == 0 && fetches) sm.dead[token] = is_dead;
                 const float poison = *bad ? __int_as_float(0x7fffffff) : 0.f;
+                if constexpr (SPLIT) {
+                    __syncwarp();
+                    cluster_wait();
+                    if (q == 0 && fetches) sm.dead[token] = is_dead;
+#pragma unroll
+                    for (int c = 0; c < C::kHalf; ++c) {
+                        const int tok = half * C::kHalf + c, owner = tok & (S - 1);
+#pragma unroll
+                        for (int b = 0; b < C::kSub; ++b)
+                            st_cluster(&sm.park[tok - owner + rank][b * 128 + wrow], owner, tot[b][c] + poison);
+                    }
+                    break;
+                }
+                // park the tile; the rows of the one before are written by now
+                asm volatile("bar.sync 1, %0;" ::"n"(kFoldWarps * 32) : "memory");
+                if (q == 0 && fetches) sm.dead[token] = is_dead;
 #pragma unroll
                 for (int b = 0; b < C::kSub; ++b)
 #pragma unroll
                     for (int c = 0; c < C::kHalf; ++c)
                         sm.park[half * C::kHalf + c][b * 128 + wrow] = tot[b][c] + poison;
-                if (SPLIT) break;
                 asm volatile("bar.sync 2, %0;" ::"n"(kFoldWarps * 32) : "memory");
                 for (int c = fw; c < NT && r0 + c < rows; c += kFoldWarps)
-                    finish_row<WR, Out>(a, t.out_vec, sm.park[c], 1, r0 + c, n0, sm.dead[c] != 0);
+                    finish_row<WR, Out, false>(a, t.out_vec, sm.park[c], 1, 0, r0 + c, n0, sm.dead[c] != 0);
             }
             __syncwarp();
         }
         if (SPLIT) {
+            // the first wait is the parking warps' own; a cluster without a tile has none of them
+            if (warp < kFoldWarp0 || !cur.more()) cluster_wait();
             cluster_sync();
-            // CTA `rank` finishes tokens rank, rank + S, ... of the cluster's tile
             if (warp >= kFoldWarp0 && cur.more()) {
                 const int64_t r0 = (int64_t)cur.rb * NT, n0 = (int64_t)cur.nt * n_step;
                 for (int c = rank + S * (warp - kFoldWarp0); c < NT && r0 + c < rows; c += S * kFoldWarps)
-                    finish_row<WR, Out>(a, t.out_vec, sm.park[c], S, r0 + c, n0, sm.dead[c] != 0);
+                    finish_row<WR, Out, false>(a, t.out_vec, sm.park[c - rank], S, C::kPitch, r0 + c, n0,
+                                               sm.dead[c] != 0);
             }
-            cluster_sync();  // no CTA leaves, or parks its next tile, while this one is read
             cur.next();
+            if (cur.more()) cluster_arrive();  // this tile is read: awaited before the next is parked
         }
     } while (SPLIT && cur.more());
     // after a wait that gave up: leave no copy in flight
@@ -350,7 +373,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::);
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sm.tmem_base), "r"(C::kTmemCols));
     }
 }
 

@@ -15,8 +15,8 @@
 //   warps 2, 3 copy the x rows of routed tiles with cp.async instead; warp 3 sends finished 16- and
 //              32-bit outputs by TMA.
 //   warps 4-11 fold: lane quarter warp % 4, one half of the columns each; then the epilogue. They
-//              take the registers that the first four warps give back (setmaxnreg; 128 x 72 +
-//              256 x 216 = 384 x 168, what the block was launched with).
+//              take registers that the first four warps give back (setmaxnreg: 128 x 64 + 256 x 216
+//              = 63,488 of the 384 x 168 = 64,512 that the block was launched with).
 //
 // When there are fewer tiles than SMs, a cluster of S CTAs shares a tile: each takes a slice of
 // the K blocks, parks its fp32 partial tile in shared memory, and after a cluster barrier CTA r
@@ -185,21 +185,24 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         prefetch_map(&tmx);
         prefetch_map(&tmw);
     }
-    if (tid == 0) {
-        sm.bad = 0;
-        for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(&sm.full[s], copy_rows ? 1 + kGatherWarps : 1);
-            mbar_init(&sm.empty[s], 1);
+    // The producer sets up its barriers and goes on to its first copies; the others meet when the
+    // tensor memory is there too.
+    if (warp == 0) {
+        if (lane == 0) sm.bad = 0;
+        if (lane < C::kStages) {
+            mbar_init(&sm.full[lane], copy_rows ? 1 + kGatherWarps : 1);
+            mbar_init(&sm.empty[lane], 1);
         }
-        for (int s = 0; s < C::kAcc; ++s) {
-            mbar_init(&sm.tfull[s], 1);
-            mbar_init(&sm.tempty[s], kFoldWarps);
+        if (lane < C::kAcc) {
+            mbar_init(&sm.tfull[lane], 1);
+            mbar_init(&sm.tempty[lane], kFoldWarps);
         }
-        for (int s = 0; s < 2 * C::kLines; ++s) {
-            mbar_init(&sm.ofull[s], 4);  // the four lane quarters
-            mbar_init(&sm.ofree[s], 1);
+        if (lane < 2 * C::kLines) {
+            mbar_init(&sm.ofull[lane], 4);  // the four lane quarters
+            mbar_init(&sm.ofree[lane], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        __syncwarp();
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -207,17 +210,20 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                      "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::);
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::);
-    const uint32_t tmem = sm.tmem_base;
+    if (warp == 0) {
+        asm volatile("bar.arrive 8, %0;" ::"n"(kThreads) : "memory");
+    } else {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::);
+        asm volatile("bar.sync 8, %0;" ::"n"(kThreads) : "memory");
+        asm volatile("tcgen05.fence::after_thread_sync;" ::);
+    }
 
     // One pass runs all of the CTA's tiles, every role at its own pace; with a split it is one tile,
     // and the cluster meets before the next. Each role keeps its ring positions over the passes.
     uint32_t issued = 0;
     Walk cur = first;
     if (warp < kFoldWarp0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         Ring<C::kStages> st;
         Ring<C::kAcc> tb;
         do {
@@ -265,7 +271,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                             if (!room) mbar_wait(&sm.tempty[tb.idx], tb.phase ^ 1, bad);
                             asm volatile("tcgen05.fence::after_thread_sync;" ::);
                             const uint32_t xa = smem_u32(sm.ring[st.idx]);
-                            const uint32_t d = tmem + tb.idx * BN;
+                            const uint32_t d = sm.tmem_base + tb.idx * BN;
                             const uint32_t stage_done = smem_u32(&sm.empty[st.idx]);
                             const uint32_t acc_done = smem_u32(&sm.tfull[tb.idx]);
                             st.next();
@@ -405,6 +411,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         } while (SPLIT && cur.more());
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const uint32_t tmem = sm.tmem_base;
         Ring<C::kAcc> tb;
         do {
             // ---------------- fold + epilogue ----------------
@@ -594,7 +601,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     const float* part = reinterpret_cast<const float*>(sm.ring);
                     for (int tr = rank + S * (warp - kFoldWarp0); tr < kRows && r0 + tr < rows;
                          tr += S * kFoldWarps)
-                        finish_row<BN, Out>(a, t.out_vec, part + tr * C::kPitch, S, r0 + tr, n0, false);
+                        finish_row<BN, Out, true>(a, t.out_vec, part + tr * C::kPitch, S, 0, r0 + tr, n0, false);
                 }
                 // no CTA leaves, or loads its next tile over the parked one, while that is read
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -615,7 +622,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::);
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sm.tmem_base), "r"(512u));
     }
 }
 
