@@ -663,7 +663,8 @@ bool fp8_tc_ok(const Fp8Args& a) {
 int launch_fp8_tc(const Fp8Args& a, cudaStream_t st) {
     // Up to 64 rows a block the tokens go on the MMA's N side, where they cost by their number.
     const int64_t rows = a.expert_ids ? a.block_m : a.P;
-    if (rows <= 64) return launch_fp8_swap(a, st);
+    if (rows <= 64 || (!a.expert_ids && (rows + 63) / 64 * ((a.N + 127) / 128) <= sm_count()))
+        return launch_fp8_swap(a, st);
     TcArgs t{};
     t.f = a;
     t.tile_rows = kRows;
