@@ -7,6 +7,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -246,11 +247,23 @@ __device__ __forceinline__ void finish_row(const Fp8Args& a, bool vec, const flo
     }
 }
 
+constexpr int kMaxDevices = 64;
+
+inline int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+// The current device's SM count, asked for once.
 inline int sm_count() {
-    int dev = 0, n = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n > 0 ? n : 148;
+    static std::atomic<int> known[kMaxDevices];
+    const int dev = current_device();
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        n = n > 0 ? n : 148;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 
 // Tensor maps of both kernels: x rows in boxes of x_box (1: gathered), weight rows as (slab, row,
@@ -282,11 +295,16 @@ inline bool out_vec(const Fp8Args& a) {
 }
 
 // Persistent launch of `tiles` tiles over clusters of t.split CTAs.
-template <typename Kernel, typename... Maps>
-int launch_persistent(Kernel kern, const TcArgs& t, int64_t tiles, size_t smem, cudaStream_t st,
-                      const Maps&... maps) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
+template <auto kKernel, typename... Maps>
+int launch_persistent(const TcArgs& t, int64_t tiles, size_t smem, cudaStream_t st, const Maps&... maps) {
+    static std::atomic<bool> ready[kMaxDevices];  // this kernel's shared-memory limit is set
+    const int dev = current_device();
+    cudaError_t e;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return (int)e;
+        ready[dev].store(true, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, std::max(1, sm_count() / t.split)) * t.split));
     cfg.blockDim = dim3(kThreads);
@@ -297,7 +315,7 @@ int launch_persistent(Kernel kern, const TcArgs& t, int64_t tiles, size_t smem, 
     at[0].val.clusterDim = {(unsigned)t.split, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = t.split > 1 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, t, maps...);
+    e = cudaLaunchKernelEx(&cfg, kKernel, t, maps...);
     return e != cudaSuccess ? (int)e : launch_status();
 }
 

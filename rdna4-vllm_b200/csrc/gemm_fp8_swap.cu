@@ -383,8 +383,8 @@ int launch_t(const TcArgs& t, int64_t tiles, cudaStream_t st) {
     CUtensorMap tmx, tmw;
     if (!make_maps(t.f, t.f.sorted_ids ? 1 : NT, WR, &tmx, &tmw))
         return set_error("fp8_block: tensor map encoding failed");
-    return launch_persistent(fp8_swap_kernel<NT, WR, Out, SPLIT>, t, tiles,
-                             sizeof(Smem<NT, WR>) + 1024, st, tmx, tmw);
+    return launch_persistent<fp8_swap_kernel<NT, WR, Out, SPLIT>>(t, tiles, sizeof(Smem<NT, WR>) + 1024,
+                                                                  st, tmx, tmw);
 }
 
 template <int NT, typename Out>

@@ -386,10 +386,7 @@ struct NormArgs {
 
 template <typename T, typename W, int kThreads, int V>
 int launch_norm_vec(const NormArgs& a, cudaStream_t st) {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const int64_t most = (int64_t)sms * (2048 / kThreads);
+    const int64_t most = (int64_t)148 * (2048 / kThreads);  // CTAs that fill the GPU
     rms_norm_quant_vec_kernel<T, W, kThreads, V><<<(unsigned)(a.M < most ? a.M : most), kThreads, 0, st>>>(
         static_cast<const T*>(a.x), static_cast<const T*>(a.residual),
         static_cast<const W*>(a.weight), a.eps, a.M, (uint32_t)a.H,

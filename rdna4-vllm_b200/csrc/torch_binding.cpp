@@ -512,13 +512,15 @@ at::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tenso
     return at::detail::empty_cuda(sizes, dtype, x.device(), c10::nullopt);
 }
 
-std::vector<at::Tensor> act_quant_fp8_block_forward(const at::Tensor& x) {
-    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(),
-                "x must be a contiguous (M, K) CUDA tensor");
+// x, residual and weight of these two may have any strides: they are activations and one vector.
+std::vector<at::Tensor> act_quant_fp8_block_forward(const at::Tensor& x_) {
+    TORCH_CHECK(x_.is_cuda() && x_.dim() == 2, "x must be an (M, K) CUDA tensor");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const auto xc = x_.expect_contiguous();
+    const at::Tensor& x = *xc;
     const int32_t dt = dtype_code(x.scalar_type(), "x");
     const int64_t M = x.size(0), K = x.size(1);
     TORCH_CHECK(K > 0, "x must have at least one column");
-    const c10::cuda::CUDAGuard guard(x.device());
     auto q = new_cuda({M, K}, at::kFloat8_e4m3fn, x);
     auto s = new_cuda({M, scale_blocks(K)}, at::kFloat, x);
     check_status(w4a8_act_quant_fp8_block(x.data_ptr(), dt, M, K, static_cast<uint8_t*>(q.data_ptr()),
@@ -528,25 +530,30 @@ std::vector<at::Tensor> act_quant_fp8_block_forward(const at::Tensor& x) {
 }
 
 // Returns {q, scales, residual_out, normed}; an output that was not asked for is an empty tensor.
-std::vector<at::Tensor> rms_norm_quant_fp8_forward(const at::Tensor& x, const at::Tensor& weight,
+std::vector<at::Tensor> rms_norm_quant_fp8_forward(const at::Tensor& x_, const at::Tensor& weight_,
                                                    double eps,
-                                                   const c10::optional<at::Tensor>& residual,
+                                                   const c10::optional<at::Tensor>& residual_,
                                                    bool with_normed) {
-    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(),
-                "x must be a contiguous (M, H) CUDA tensor");
+    TORCH_CHECK(x_.is_cuda() && x_.dim() == 2, "x must be an (M, H) CUDA tensor");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const auto xc = x_.expect_contiguous();
+    const auto wc = weight_.expect_contiguous();
+    const at::Tensor &x = *xc, &weight = *wc;
     const int32_t dt = dtype_code(x.scalar_type(), "x");
     const int64_t M = x.size(0), H = x.size(1);
     TORCH_CHECK(H > 0, "x must have at least one column");
-    TORCH_CHECK(weight.device() == x.device() && weight.dim() == 1 && weight.size(0) == H &&
-                    weight.is_contiguous(),
-                "weight must be a contiguous (H,) tensor on x's device");
+    TORCH_CHECK(weight.device() == x.device() && weight.dim() == 1 && weight.size(0) == H,
+                "weight must be an (H,) tensor on x's device");
     TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
                 "weight must have x's type or fp32");
-    if (residual)
-        TORCH_CHECK(residual->device() == x.device() && residual->sizes() == x.sizes() &&
-                        residual->scalar_type() == x.scalar_type() && residual->is_contiguous(),
-                    "residual must be contiguous with x's shape, type and device");
-    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor res_in;
+    if (residual_) {
+        TORCH_CHECK(residual_->device() == x.device() && residual_->sizes() == x.sizes() &&
+                        residual_->scalar_type() == x.scalar_type(),
+                    "residual must have x's shape, type and device");
+        res_in = residual_->contiguous();
+    }
+    const bool residual = res_in.defined();
     auto q = new_cuda({M, H}, at::kFloat8_e4m3fn, x);
     auto s = new_cuda({M, scale_blocks(H)}, at::kFloat, x);
     auto res = new_cuda({residual ? M : 0, H}, x.scalar_type(), x);
@@ -554,7 +561,7 @@ std::vector<at::Tensor> rms_norm_quant_fp8_forward(const at::Tensor& x, const at
     // an empty batch has no storage to point at; there is nothing to launch either
     if (M > 0)
         check_status(w4a8_rms_norm_quant_fp8(
-                         x.data_ptr(), residual ? residual->data_ptr() : nullptr,
+                         x.data_ptr(), residual ? res_in.data_ptr() : nullptr,
                          weight.data_ptr(), dt, dtype_code(weight.scalar_type(), "weight"),
                          (float)eps, M, H, static_cast<uint8_t*>(q.data_ptr()),
                          s.data_ptr<float>(), residual ? res.data_ptr() : nullptr,

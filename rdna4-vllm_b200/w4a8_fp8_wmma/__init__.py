@@ -190,7 +190,7 @@ _fp8_block_moe_gemm1_silu_op = torch.ops.w4a8_b200.fp8_block_moe_gemm1_silu.defa
 def act_quant_fp8_block(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(M, K) fp16/bf16/fp32 -> (q (M, K) float8_e4m3fn, scales (M, ceil(K/128)) fp32): the rule
     of act_quant_fp8 applied to each 128 columns of a row."""
-    return tuple(_act_quant_fp8_block_op(x.contiguous()))
+    return tuple(_act_quant_fp8_block_op(x))
 
 
 def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -202,9 +202,7 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     residual or None, y in x's type if with_normed else None). x and residual fp16, bf16 or
     fp32; weight in x's type or fp32.
     """
-    q, s, res, normed = _rms_norm_quant_fp8_op(
-        x.contiguous(), weight.contiguous(), float(eps),
-        residual.contiguous() if residual is not None else None, bool(with_normed))
+    q, s, res, normed = _rms_norm_quant_fp8_op(x, weight, eps, residual, with_normed)
     return q, s, (res if residual is not None else None), (normed if with_normed else None)
 
 
@@ -229,9 +227,8 @@ def fp8_block_moe_gemm(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
     None: x has P rows that are already in sorted order. Returns (P, N); padding rows and rows of
     an expert id outside [0, E) are zero, rows past num_tokens_post_padded are not written.
     """
-    return _fp8_block_moe_gemm_op(
-        x, x_scales, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded,
-        int(top_k), int(block_m), out_dtype)
+    return _fp8_block_moe_gemm_op(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
+                                  num_tokens_post_padded, top_k, block_m, out_dtype)
 
 
 def fp8_block_moe_gemm1_silu(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
@@ -242,10 +239,8 @@ def fp8_block_moe_gemm1_silu(x, x_scales, w, w_scales, sorted_token_ids, expert_
     reads for the down product. silu(gate) * up is evaluated in fp32 and rounded once, to e4m3.
     inter must be a multiple of 128; the rest as fp8_block_moe_gemm.
     """
-    q, s = _fp8_block_moe_gemm1_silu_op(
-        x, x_scales, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded,
-        int(top_k), int(block_m))
-    return q, s
+    return tuple(_fp8_block_moe_gemm1_silu_op(x, x_scales, w, w_scales, sorted_token_ids,
+                                              expert_ids, num_tokens_post_padded, top_k, block_m))
 
 
 # ---- Fake / meta impls (output contracts of the CUDA impls, reference __init__.py:240-297) ----

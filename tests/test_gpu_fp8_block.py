@@ -121,6 +121,18 @@ def test_rms_norm_quant_edges(w4):
     assert q.shape == (0, 256) and s.shape == (0, 2) and res.shape == (0, 256) and n.shape == (0, 256)
 
 
+def test_quantisers_take_strided_rows(w4):
+    g = _gen(10)
+    wide = _randn(g, 6, 3 * 256, dtype=BF16)
+    x, r, w = wide[:, 256:512], wide[:, 512:], _randn(g, 512, dtype=BF16)[::2]
+    for a, b in zip(w4.act_quant_fp8_block(x), w4.act_quant_fp8_block(x.contiguous())):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    ours = w4.rms_norm_quant_fp8(x, w, 1e-6, residual=r, with_normed=True)
+    ref = w4.rms_norm_quant_fp8(x.contiguous(), w.contiguous(), 1e-6, residual=r.contiguous(), with_normed=True)
+    for a, b in zip(ours, ref):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_rms_norm_quant_residual_in_place(w4):
     """The C entry may be given the residual itself as the new residual."""
     g = _gen(9)
