@@ -61,6 +61,22 @@ struct Walk {
     }
 };
 
+// A load that stays where it is written: fetched a tile ahead of its use, it would otherwise be
+// moved down to it to save a register.
+__device__ __forceinline__ float fetch(const float* p) {
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int fetch(const int32_t* p) {
+    int v;
+    asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 // x's row of output row r, or -1 when r is a row of zeros (absent expert e, padding slot).
 __device__ __forceinline__ int64_t source_row(const Fp8Args& a, int64_t r, int64_t rows, int e) {
     if (r >= rows || e < 0 || e >= a.E) return -1;

@@ -14,8 +14,9 @@
 // written by whole warps (fp8_tc.cuh: finish_row).
 //
 // One persistent CTA per SM, 12 warps: 0 TMA producer (x rows by a 2D box, or by tile::gather4
-// through the routing, 4 rows a lane), 1 tensor memory and MMA issue, 2 and 3 idle (a lane quarter
-// needs warps 4 k + q), 4-11 fold: lane quarter warp % 4, one half of the tokens each. With few
+// through the routing, 4 rows a lane), 1 tensor memory and MMA issue, 2 and 3 write the rows of a
+// parked tile while the next is folded (tiles of up to 32 tokens; with the fold warps doing it a
+// tile of 4 blocks spent half its time there), 4-11 fold: lane quarter warp % 4, one half of the tokens each. With few
 // tiles a cluster of S CTAs shares one along K: token c belongs to CTA c % S, every CTA parks its
 // part of it there (distributed shared memory), and after a cluster barrier the owner adds the parts
 // in rank order.
@@ -37,10 +38,15 @@ struct Cfg {
     static constexpr int kAccCols = kSub * NT; // tensor-memory columns of a block of K
     static constexpr int kAcc = 4;
     static constexpr int kPitch = WR + 4;      // floats per token of a parked tile
+    static constexpr bool kAside = NT <= 32;   // finished by warps 2 and 3
     static constexpr int kPark = NT * kPitch * 4;
     static constexpr int kFree = 227 * 1024 - 1024 - 2048 - kPark - 2 * kFoldWarps * kSub * kHalf * 4;
     static constexpr int kMost = kFree / (int)(kWBytes + kXBytes);
-    static constexpr int kStages = kMost < 12 ? kMost : 12;
+    // A full memory system is not served faster by more requests, and the scales' own loads queue
+    // behind them: down at 32 tokens takes 39.2, 34.8, 34.7 and 36.2 us with 2, 3, 4 and 6 stages of
+    // 256 weight rows. Narrow tiles, where a CTA has one, take what there is.
+    static constexpr int kCap = WR == 256 ? 4 : 12;
+    static constexpr int kStages = kMost < kCap ? kMost : kCap;
     static constexpr uint32_t kTmemCols = kAcc * kAccCols < 32 ? 32 : kAcc * kAccCols;
 };
 
@@ -52,6 +58,7 @@ struct Smem {
     float scale[2][kFoldWarps][C::kSub][C::kHalf];      // [block parity][warp]: xs * ws of its tokens
     uint64_t full[C::kStages], empty[C::kStages];
     uint64_t tfull[C::kAcc], tempty[C::kAcc];
+    uint64_t parked, read;                              // the parked tile, when it is finished aside
     int dead[NT];                                       // tokens whose row is one of zeros
     uint32_t tmem_base;
     int bad;
@@ -90,6 +97,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     const Fp8Args& a = t.f;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* bad = &sm.bad;
+    const int* some_int = reinterpret_cast<const int*>(a.ws);  // can be read; holds at least one
 
     const int S = SPLIT ? t.split : 1;
     const int rank = SPLIT ? (int)cluster_rank() : 0;
@@ -99,7 +107,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     const int g_lo = (int)((int64_t)G * rank / S), g_hi = (int)((int64_t)G * (rank + 1) / S);
     const int n_step = SILU ? 128 : WR;  // outputs per tile
     const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
-    auto expert_of = [&](int rb) { return a.expert_ids ? a.expert_ids[rb] : 0; };
+    auto expert_of = [&](int rb) { return a.expert_ids ? fetch(a.expert_ids + rb) : 0; };
 
     if (tid == 32 * 2) {
         prefetch_map(&tmx);
@@ -116,6 +124,10 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         if (lane < C::kAcc) {
             mbar_init(&sm.tfull[lane], 1);
             mbar_init(&sm.tempty[lane], kFoldWarps);
+        }
+        if (lane == 0) {
+            mbar_init(&sm.parked, kFoldWarps);
+            mbar_init(&sm.read, 2);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         __syncwarp();
@@ -152,7 +164,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int64_t r = (int64_t)w.rb * NT + 4 * lane + i;
-                    slot[i] = a.sorted_ids && 4 * lane < NT && r < rows ? a.sorted_ids[r] : -1;
+                    slot[i] = a.sorted_ids && 4 * lane < NT && r < rows ? fetch(a.sorted_ids + r) : -1;
                 }
             };
             Walk w = cur;
@@ -223,71 +235,97 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 }
             }
             __syncwarp();
-        } else if (warp >= kFoldWarp0) {
+        } else if (warp < kFoldWarp0) {
+            // ---------------- rows of a parked tile ----------------
+            if (C::kAside && !SPLIT) {
+                uint32_t turn = 0;
+                for (Walk w = cur; w.more(); w.next(), turn ^= 1) {
+                    const int64_t r0 = (int64_t)w.rb * NT, n0 = (int64_t)w.nt * n_step;
+                    mbar_wait(&sm.parked, turn, bad);
+                    for (int c = warp - 2; c < NT && r0 + c < rows; c += 2)
+                        finish_row<WR, Out, false>(a, t.out_vec, sm.park[c], 1, 0, r0 + c, n0, sm.dead[c] != 0);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.read);
+                }
+                __syncwarp();
+            }
+        } else {
             // ---------------- fold + epilogue ----------------
             const int q = warp & 3, fw = warp - kFoldWarp0, half = fw >> 2;
             const int wrow = q * 32 + lane;                // weight row within a 128-row accumulator
             const int token = half * C::kHalf + lane;      // whose scale this lane fetches
             const bool fetches = lane < C::kHalf;
             const int64_t NB = (a.N + kBlk - 1) / kBlk;
-            // a tile's first scales are fetched while the tile before it folds its last block, its
-            // routing entries a whole tile ahead
-            const float *xs = a.xs, *ws0 = a.ws, *ws1 = a.ws;
-            float sx = 0.f, s0 = 0.f, s1 = 0.f;
-            bool present = false, dead = true;
-            int next_e = -1, next_slot = -1;
-            auto look = [&](const Walk& w) {
-                if (!w.more()) return;
-                const int64_t r = (int64_t)w.rb * NT + token;
-                next_e = expert_of(w.rb);
-                next_slot = !fetches || r >= rows ? -1 : a.sorted_ids ? a.sorted_ids[r] : (int)r;
+            // With the weights streaming, a load from memory takes as long as a short tile: a tile's
+            // first scales are fetched one tile ahead, its routing entries two. The fetches are
+            // unconditional (from some address that can be read, where there is nothing to fetch),
+            // since a value merged behind a branch is waited for at the merge.
+            struct Scales {
+                const float *xs, *ws0, *ws1;  // this lane's token's, and its weight blocks'
+                float x, w0, w1;              // of the next block of K
+                bool present, dead;
             };
-            auto enter = [&](const Walk& w) {
-                const int e = next_e;
-                present = e >= 0 && e < a.E;
-                int src = next_slot;
+            Scales now, ahead;
+            uint32_t turn = 0;  // phase of the parked tile
+            int next_e = -1, next_slot = -1;
+            auto row_of = [&](const Walk& w) { return (int64_t)w.rb * NT + token; };
+            auto look = [&](const Walk& w) {
+                const int64_t r = row_of(w);
+                next_e = fetch(a.expert_ids && w.more() ? a.expert_ids + w.rb : some_int);
+                next_slot = fetch(a.sorted_ids && fetches && r < rows ? a.sorted_ids + r : some_int);
+            };
+            auto enter = [&](const Walk& w, Scales& s) {
+                const int e = a.expert_ids ? next_e : 0;
+                s.present = w.more() && e >= 0 && e < a.E && g_lo < g_hi;
+                const int64_t r = row_of(w);
+                int src = fetches && r < rows ? (a.sorted_ids ? next_slot : (int)r) : -1;
                 if (a.sorted_ids) src = src >= 0 && src < a.num_slots ? src / a.top_k : -1;
-                dead = !present || src < 0;
-                if (!present) return;
+                s.dead = !s.present || src < 0;
                 const int64_t b0 = (int64_t)w.nt * n_step / kBlk;
-                xs = a.xs + (int64_t)max(src, 0) * G;
-                ws0 = a.ws + (e * NB + b0) * G;
-                ws1 = SILU ? ws0 + (a.N / 2 / kBlk) * G : a.ws + (e * NB + min(b0 + 1, NB - 1)) * G;
-                if (g_lo < g_hi) {
-                    sx = __ldg(xs + g_lo);
-                    s0 = __ldg(ws0 + g_lo);
-                    if (C::kSub == 2) s1 = __ldg(ws1 + g_lo);
+                const float* ws = a.ws + (s.present ? e * NB * G : 0);
+                s.xs = a.xs + (s.dead ? 0 : src * (int64_t)G);
+                s.ws0 = ws + (s.present ? b0 * G : 0);
+                s.ws1 = ws + (s.present ? (SILU ? b0 + a.N / 2 / kBlk : min(b0 + 1, NB - 1)) * G : 0);
+                s.x = fetch(s.xs + g_lo);
+                s.w0 = fetch(s.ws0 + g_lo);
+                s.w1 = C::kSub == 2 ? fetch(s.ws1 + g_lo) : 0.f;
+                for (int g = g_lo + 8; g < g_hi; g += 8) {  // 32 bytes at a time
+                    if (fetches) prefetch_l2(s.xs + g);
+                    if (lane == 0) prefetch_l2(s.ws0 + g);
+                    if (C::kSub == 2 && lane == 0) prefetch_l2(s.ws1 + g);
                 }
             };
-            Walk w = cur;
+            Walk w = cur, w1 = cur;  // the tile, and the next
             look(w);
-            if (w.more()) enter(w);
+            enter(w, now);
+            w1.next();
+            if (!SPLIT) look(w1);
             while (w.more()) {
                 const int64_t r0 = (int64_t)w.rb * NT, n0 = (int64_t)w.nt * n_step;
-                const bool is_dead = dead, is_present = present && g_lo < g_hi;
-                w.next();
-                if (!SPLIT) look(w);
+                const bool is_dead = now.dead;
+                w = w1;
+                if (!SPLIT) {
+                    enter(w, ahead);
+                    w1.next();
+                    look(w1);
+                }
                 float tot[C::kSub][C::kHalf];
 #pragma unroll
                 for (int b = 0; b < C::kSub; ++b)
 #pragma unroll
                     for (int c = 0; c < C::kHalf; ++c) tot[b][c] = 0.f;
-                if (!is_present && !SPLIT && w.more()) enter(w);
-                if (is_present) {
+                if (now.present) {
 #pragma unroll 1
                     for (int g = g_lo; g < g_hi; ++g) {
                         float(&sc)[C::kSub][C::kHalf] = sm.scale[g & 1][fw];
                         if (fetches) {
-                            sc[0][lane] = sx * s0;
-                            if (C::kSub == 2) sc[C::kSub - 1][lane] = sx * s1;
+                            sc[0][lane] = now.x * now.w0;
+                            if (C::kSub == 2) sc[C::kSub - 1][lane] = now.x * now.w1;
                         }
-                        if (g + 1 < g_hi) {  // the next block's scales, behind this block's fold
-                            sx = __ldg(xs + g + 1);
-                            s0 = __ldg(ws0 + g + 1);
-                            if (C::kSub == 2) s1 = __ldg(ws1 + g + 1);
-                        } else if (!SPLIT && w.more()) {
-                            enter(w);
-                        }
+                        const int next_g = min(g + 1, g_hi - 1);  // behind this block's fold
+                        now.x = fetch(now.xs + next_g);
+                        now.w0 = fetch(now.ws0 + next_g);
+                        if (C::kSub == 2) now.w1 = fetch(now.ws1 + next_g);
                         __syncwarp();
                         mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::);
@@ -333,17 +371,28 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     }
                     break;
                 }
-                // park the tile; the rows of the one before are written by now
-                asm volatile("bar.sync 1, %0;" ::"n"(kFoldWarps * 32) : "memory");
+                // park the tile once the rows of the one before are written
+                if (C::kAside) {
+                    mbar_wait(&sm.read, turn ^ 1, bad);
+                    turn ^= 1;
+                } else {
+                    asm volatile("bar.sync 1, %0;" ::"n"(kFoldWarps * 32) : "memory");
+                }
                 if (q == 0 && fetches) sm.dead[token] = is_dead;
 #pragma unroll
                 for (int b = 0; b < C::kSub; ++b)
 #pragma unroll
                     for (int c = 0; c < C::kHalf; ++c)
                         sm.park[half * C::kHalf + c][b * 128 + wrow] = tot[b][c] + poison;
-                asm volatile("bar.sync 2, %0;" ::"n"(kFoldWarps * 32) : "memory");
-                for (int c = fw; c < NT && r0 + c < rows; c += kFoldWarps)
-                    finish_row<WR, Out, false>(a, t.out_vec, sm.park[c], 1, 0, r0 + c, n0, sm.dead[c] != 0);
+                if (C::kAside) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.parked);
+                } else {
+                    asm volatile("bar.sync 2, %0;" ::"n"(kFoldWarps * 32) : "memory");
+                    for (int c = fw; c < NT && r0 + c < rows; c += kFoldWarps)
+                        finish_row<WR, Out, false>(a, t.out_vec, sm.park[c], 1, 0, r0 + c, n0, sm.dead[c] != 0);
+                }
+                if (!SPLIT) now = ahead;
             }
             __syncwarp();
         }
