@@ -328,6 +328,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         if (C::kSub == 2) now.w1 = fetch(now.ws1 + next_g);
                         __syncwarp();
                         mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
+                        __syncwarp();
                         asm volatile("tcgen05.fence::after_thread_sync;" ::);
                         const uint32_t base =
                             sm.tmem_base + ((uint32_t)(q * 32) << 16) + tb.idx * C::kAccCols + half * C::kHalf;

@@ -84,10 +84,10 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
 }
 
 // One block's accumulator into the running totals: columns col(0..kCols) at `base`, the first half
-// scaled by f0 and the second by f1.
-template <int kCols, typename Col>
+// scaled by f0 and the second by f1; released() runs when the last columns are in registers.
+template <int kCols, typename Col, typename Done>
 __device__ __forceinline__ void fold_block(uint32_t base, Col col, float f0, float f1,
-                                           float (&tot)[kCols]) {
+                                           float (&tot)[kCols], Done released) {
     uint32_t v[2][16];
     tmem_ld16_nowait(base + col(0), v[0]);
     tmem_wait16(v[0]);
@@ -96,6 +96,7 @@ __device__ __forceinline__ void fold_block(uint32_t base, Col col, float f0, flo
         uint32_t(&now)[16] = v[(j / 16) & 1];
         uint32_t(&next)[16] = v[(j / 16 + 1) & 1];
         if (j + 16 < kCols) tmem_ld16_nowait(base + col(j + 16), next);
+        else released();
         const float f = j < kCols / 2 ? f0 : f1;
         const float2 f2 = make_float2(f, f);
 #pragma unroll
@@ -179,7 +180,13 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     constexpr int kLineCols = 128 / kOutSize;                      // columns of a staged line
     constexpr int kRounds = C::kCols / (C::kLines * kLineCols);    // staging areas per tile
     const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
-    auto expert_of = [&](int rb) { return a.expert_ids ? a.expert_ids[rb / per_expert] : 0; };
+    // expert of w's row block, fetched without a branch (a value merged behind one is waited for at
+    // the merge); no expert where there is no such tile
+    const int* some_int = reinterpret_cast<const int*>(a.ws);  // can be read; holds at least one
+    auto fetch_expert = [&](const Walk& w) {
+        return fetch(a.expert_ids && w.more() ? a.expert_ids + w.rb / per_expert : some_int);
+    };
+    auto expert = [&](int fetched) { return a.expert_ids ? fetched : 0; };
 
     if (tid == 32 * 2) {
         prefetch_map(&tmx);
@@ -230,15 +237,13 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             if (warp == 0) {
                 // ---------------- TMA producer ----------------
                 const uint32_t stage_bytes = (copy_rows ? 0u : (uint32_t)kRows * 128) + C::kBBytes;
-                for (Walk w = cur; w.more(); w.next()) {
-                    const int e = expert_of(w.rb);
-                    if (e < 0 || e >= a.E) {
-                        if (SPLIT) break;
-                        continue;
-                    }
-                    const int r0 = w.rb * kRows;
-                    const int w_row = w.nt * n_step, w_slab = SILU ? 2 * e : e;
-                    for (int g = g_lo; g < g_hi; ++g) {
+                Walk w = cur;
+                int next_e = fetch_expert(w);
+                while (w.more()) {
+                    const int e = expert(next_e), r0 = w.rb * kRows, w_row = w.nt * n_step, w_slab = SILU ? 2 * e : e;
+                    w.next();
+                    if (!SPLIT) next_e = fetch_expert(w);
+                    for (int g = e >= 0 && e < a.E ? g_lo : g_hi; g < g_hi; ++g) {
                         uint8_t* xa = sm.ring[st.idx];
                         uint64_t* fb = &sm.full[st.idx];
                         if (elect_one()) {
@@ -260,13 +265,13 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 if (elect_one()) {
                     constexpr uint32_t idesc = umma_idesc(128, BN);
                     bool full = false, room = false;  // the next block's barriers were seen complete
-                    for (Walk w = cur; w.more(); w.next()) {
-                        const int e = expert_of(w.rb);
-                        if (e < 0 || e >= a.E) {
-                            if (SPLIT) break;
-                            continue;
-                        }
-                        for (int g = g_lo; g < g_hi; ++g) {
+                    Walk w = cur;
+                    int next_e = fetch_expert(w);
+                    while (w.more()) {
+                        const int e = expert(next_e);
+                        w.next();
+                        if (!SPLIT) next_e = fetch_expert(w);
+                        for (int g = e >= 0 && e < a.E ? g_lo : g_hi; g < g_hi; ++g) {
                             if (!full) mbar_wait(&sm.full[st.idx], st.phase, bad);
                             if (!room) mbar_wait(&sm.tempty[tb.idx], tb.phase ^ 1, bad);
                             asm volatile("tcgen05.fence::after_thread_sync;" ::);
@@ -342,24 +347,25 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                     int slot[kSlots], e = -1;
                     auto row_of = [&](int i) { return (i >> 2) * 4 * kGatherWarps + (warp - 2) * 4 + (i & 3); };
                     auto look = [&](const Walk& w) {
-                        if (!w.more()) return;
-                        e = expert_of(w.rb);
+                        e = fetch_expert(w);
 #pragma unroll
                         for (int i = 0; i < kSlots; ++i) {
-                            const int tr = row_of(lane + 32 * i);
-                            const int64_t r = (int64_t)w.rb * kRows + tr;
-                            slot[i] = r < rows ? a.sorted_ids[r] : -1;
+                            const int64_t r = (int64_t)w.rb * kRows + row_of(lane + 32 * i);
+                            slot[i] = fetch(r < rows ? a.sorted_ids + r : some_int);
                         }
                     };
                     Walk w = cur;
                     look(w);
                     while (w.more()) {
-                        const bool present = e >= 0 && e < a.E;
+                        const bool present = expert(e) >= 0 && expert(e) < a.E;
                         __syncwarp();
 #pragma unroll
                         for (int i = 0; i < kSlots; ++i)
                             sm.src[row_of(lane + 32 * i)] =
-                                slot[i] >= 0 && slot[i] < a.num_slots ? slot[i] / a.top_k : -1;
+                                (int64_t)w.rb * kRows + row_of(lane + 32 * i) < rows && slot[i] >= 0 &&
+                                        slot[i] < a.num_slots
+                                    ? slot[i] / a.top_k
+                                    : -1;
                         __syncwarp();
                         int src[kRowsPer <= 16 ? kRowsPer : 1];  // or from shared memory each time
                         if (kRowsPer <= 16)
@@ -417,7 +423,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             // ---------------- fold + epilogue ----------------
             const int q = warp & 3, fw = warp - kFoldWarp0, half = fw >> 2;
             const int row = q * 32 + lane;
-            if (q * 32 < kRows) {
+            {
                 // column of tot[j]: the plain form's half is contiguous; the SiLU form's holds 64
                 // gate columns, then the 64 matching up columns
                 auto col = [&](int j) {
@@ -425,67 +431,71 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 };
                 const int64_t NB = (a.N + kBlk - 1) / kBlk;
                 int done = 0, turn = 0;  // turn: phase of the staging area
-                // The scales of a tile's first block are fetched while the tile before it folds its
-                // last one, its routing entries a whole tile ahead: neither wait is paid per tile.
+                // Scales are fetched a block of K ahead, over the tiles' borders, routing entries a whole
+                // tile ahead. The fetches are unconditional, see fetch_expert.
                 const float *xs = a.xs, *ws0 = a.ws, *ws1 = a.ws;
-                float sx = 0.f, s0 = 0.f, s1 = 0.f;
-                bool present = false, dead = true;  // of tile w, set by enter()
+                bool present = false, dead = true;  // of the tile that enter() was given
                 int next_e = -1, next_slot = -1;    // of the tile to enter next
                 auto look = [&](const Walk& w) {
-                    if (!w.more()) return;
                     const int64_t r = (int64_t)w.rb * kRows + row;
-                    next_e = expert_of(w.rb);
-                    next_slot = row >= kRows || r >= rows ? -1 : a.sorted_ids ? a.sorted_ids[r] : (int)r;
+                    next_e = fetch_expert(w);
+                    next_slot = fetch(a.sorted_ids && r < rows ? a.sorted_ids + r : some_int);
                 };
                 auto enter = [&](const Walk& w) {
-                    const int e = next_e;
-                    present = e >= 0 && e < a.E;
-                    int src = next_slot;
+                    const int e = expert(next_e);
+                    const int64_t r = (int64_t)w.rb * kRows + row;
+                    present = w.more() && e >= 0 && e < a.E && g_lo < g_hi;
+                    int src = r < rows ? (a.sorted_ids ? next_slot : (int)r) : -1;
                     if (a.sorted_ids) src = src >= 0 && src < a.num_slots ? src / a.top_k : -1;
                     dead = !present || src < 0;
-                    if (!present) return;
                     const int64_t n0 = (int64_t)w.nt * n_step;
                     const int64_t b0 = SILU ? n0 / kBlk : min((n0 + half * C::kCols) / kBlk, NB - 1);
-                    xs = a.xs + (int64_t)max(src, 0) * G;
-                    ws0 = a.ws + (e * NB + b0) * G;
-                    ws1 = SILU ? ws0 + (a.N / 2 / kBlk) * G : ws0;
-                    if (g_lo < g_hi) {
-                        sx = __ldg(xs + g_lo);
-                        s0 = __ldg(ws0 + g_lo);
-                        if (SILU) s1 = __ldg(ws1 + g_lo);
-                    }
+                    xs = a.xs + (dead ? 0 : src * (int64_t)G);
+                    ws0 = a.ws + (present ? (e * NB + b0) * G : 0);
+                    ws1 = SILU && present ? ws0 + (a.N / 2 / kBlk) * G : ws0;
+                };
+                float sx, s0, s1 = 0.f;
+                auto scales = [&](int g) {
+                    sx = fetch(xs + g);
+                    s0 = fetch(ws0 + g);
+                    if (SILU) s1 = fetch(ws1 + g);
                 };
                 Walk w = cur;
                 look(w);
-                if (w.more()) enter(w);
+                enter(w);
+                scales(g_lo);
+                bool ready = false;  // the next accumulator was seen complete
                 while (w.more()) {
                     const int64_t r0 = (int64_t)w.rb * kRows, r = r0 + row;
                     const int64_t n0 = (int64_t)w.nt * n_step;
-                    const bool is_dead = dead, is_present = present && g_lo < g_hi;
+                    const bool is_dead = dead, is_present = present;
                     w.next();
                     if (!SPLIT) look(w);
                     float tot[C::kCols];
 #pragma unroll
                     for (int j = 0; j < C::kCols; ++j) tot[j] = 0.f;
-                    if (!is_present && !SPLIT && w.more()) enter(w);
-                    if (is_present) {
-                        for (int g = g_lo; g < g_hi; ++g) {
-                            const float f0 = sx * s0, f1 = SILU ? sx * s1 : f0;
-                            if (g + 1 < g_hi) {  // the next block's scales, behind this block's fold
-                                sx = __ldg(xs + g + 1);
-                                s0 = __ldg(ws0 + g + 1);
-                                if (SILU) s1 = __ldg(ws1 + g + 1);
-                            } else if (!SPLIT && w.more()) {
-                                enter(w);
-                            }
-                            mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::);
-                            fold_block(tmem + ((uint32_t)(q * 32) << 16) + tb.idx * BN, col, f0, f1, tot);
+                    for (int g = is_present ? g_lo : g_hi; g < g_hi; ++g) {
+                        const float f0 = sx * s0, f1 = SILU ? sx * s1 : f0;
+                        int next_g = g + 1;
+                        if (next_g == g_hi) {
+                            next_g = g_lo;
+                            if (!SPLIT) enter(w);
+                        }
+                        scales(next_g);
+                        if (!ready) mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
+                        __syncwarp();
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::);
+                        fold_block(tmem + ((uint32_t)(q * 32) << 16) + tb.idx * BN, col, f0, f1, tot, [&] {
                             asm volatile("tcgen05.fence::before_thread_sync;" ::);
                             __syncwarp();
                             if (lane == 0) mbar_arrive(&sm.tempty[tb.idx]);
                             tb.next();
-                        }
+                            ready = mbar_test(&sm.tfull[tb.idx], tb.phase);
+                        });
+                    }
+                    if (!is_present && !SPLIT) {
+                        enter(w);
+                        scales(g_lo);
                     }
                     // rows of zeros are zero whatever the lane's accumulator held: such a lane writes
                     // `fill` over its staged row (a wait that gave up makes every row one, of NaN)
