@@ -142,7 +142,7 @@ int check_grouped(const std::string& o, const Fp8Args& a, int64_t top_k, int64_t
         return set_error(o + ": block_m must be 16, 32, 64 or a multiple of 128");
     if (a.P % block_m != 0) return set_error(o + ": P not divisible by block_m");
     if (a.P == 0) return W4A8_OK;
-    if (!a.xs || !a.w || !a.ws || !a.expert_ids || !a.ntp || (a.x_rows > 0 && !a.x))
+    if (!a.w || !a.ws || !a.expert_ids || !a.ntp || (a.x_rows > 0 && (!a.x || !a.xs)))
         return set_error(o + ": null pointer");
     if (!a.sorted_ids && a.x_rows != a.P)
         return set_error(o + ": without sorted_token_ids x must have P rows");

@@ -285,7 +285,7 @@ def test_grouped_absent_experts_and_bad_slots_give_zeros(w4):
 @pytest.mark.parametrize("bm,T", [(16, 6), (128, 150)])
 def test_rows_past_the_last_are_left(w4, bm, T):
     """Through the C entries, with prefilled outputs: rows at or past num_tokens_post_padded keep
-    what they held, and num_tokens_post_padded = 0 writes nothing."""
+    what they held, also where it ends inside a block, and 0 writes nothing."""
     g = _gen(13)
     E, k, N, K = 3, 2, 256, 384
     x, xs = _matrix(g, T, K, row_block=1)
@@ -295,7 +295,7 @@ def test_rows_past_the_last_are_left(w4, bm, T):
     lib = load_lib()
     vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
     st = torch.cuda.current_stream().cuda_stream
-    for count in (rows, 0):
+    for count in (rows, rows - 5, rows - 70 if rows > 128 else 1, 0):
         n.fill_(count)
         out = torch.full((P, N), 7.0, dtype=FP16, device="cuda")
         f = lib.w4a8_fp8_block_moe_gemm
@@ -312,7 +312,86 @@ def test_rows_past_the_last_are_left(w4, bm, T):
         assert bool((q[count:] == 9).all()) and bool((qs[count:] == 5).all())
         if count:
             want, S, _ = R.grouped(x, xs, w, ws, s, e, rows, k, bm)
-            R.check_out(out[:rows], want, S, 3, FP16)
+            R.check_out(out[:count], want[:count], S[:count], 3, FP16)
+
+
+def test_no_activations_give_zero_rows(w4):
+    """T = 0 with row blocks that hold padding only."""
+    w, ws = _matrix(_gen(14), 2, 256, 256, row_block=128)
+    x, xs = torch.empty(0, 256, dtype=torch.uint8, device="cuda"), torch.empty(0, 2, device="cuda")
+    s = torch.zeros(32, dtype=torch.int32, device="cuda")
+    e = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    n = torch.tensor([32], dtype=torch.int32, device="cuda")
+    assert bool((w4.fp8_block_moe_gemm(x, xs, w, ws, s, e, n, 2, 16) == 0).all())
+    q, _ = w4.fp8_block_moe_gemm1_silu(x, xs, w, ws, s, e, n, 2, 16)
+    assert bool((q.view(torch.uint8) == 0).all())
+
+
+def test_many_tiles_with_a_short_last_block(w4):
+    """More tiles than the GPU holds, outputs that leave by copies of 128 rows, and a count that ends
+    inside the last block: the short tile follows copies that are still being read."""
+    g = _gen(15)
+    T, E, k, N, K, bm = 3000, 2, 1, 2048, 128, 128
+    x, xs = _matrix(g, T, K, row_block=1)
+    w, ws = _matrix(g, E, N, K, row_block=128)
+    s, e, n = _routing(T, E, k, bm, 3, spare=0)
+    rows = int(n) - 60
+    n.fill_(rows)
+    for dtype in (FP16, FP32):
+        out = w4.fp8_block_moe_gemm(x, xs, w, ws, s, e, n, k, bm, out_dtype=dtype)
+        want, S, _ = R.grouped(x, xs, w, ws, s, e, rows, k, bm)
+        R.check_out(out[:rows], want, S, 1, dtype)
+
+
+def test_offsets_past_32_bits(w4):
+    """Quantisation over, and products into, more than 2^31 elements; the last rows are checked."""
+    g = _gen(16)
+    M, K = 270000, 8192
+    x = torch.zeros(M, K, dtype=BF16, device="cuda")
+    x[-3:] = _randn(g, 3, K, dtype=BF16)
+    q, s, _, n = w4.rms_norm_quant_fp8(x, torch.ones(K, dtype=BF16, device="cuda"), 1e-5, with_normed=True)
+    q2, s2, _, n2 = w4.rms_norm_quant_fp8(x[-3:], torch.ones(K, dtype=BF16, device="cuda"), 1e-5, with_normed=True)
+    assert torch.equal(q[-3:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s[-3:], s2) and torch.equal(n[-3:], n2)
+    del n, n2
+    q, s = w4.act_quant_fp8_block(x)
+    rq, rs = R.quantise(x[-3:].float())
+    assert torch.equal(q[-3:].view(torch.uint8), rq.view(torch.uint8)) and torch.equal(s[-3:], rs)
+    del x
+    w, ws = _matrix(g, 8320, 128, row_block=128)
+    out = w4.fp8_block_gemm(q[:, :128].contiguous(), s[:, :1].contiguous(), w, ws)
+    assert out.numel() > 1 << 31
+    want, S = R.product(q[-3:, :128], s[-3:, :1], w, ws)
+    R.check_out(out[-3:], want, S, 1, FP16)
+    del out
+    # activation rows past 2^31 bytes, through the routing, in both forms of the kernel
+    xw, wsw = _matrix(g, 2, 256, K, row_block=128)
+    for bm in (16, 128):
+        src = torch.tensor([M - 1, M - 2, M - 3, 5] + [M] * (bm - 4), dtype=torch.int32, device="cuda")
+        one = torch.ones(1, dtype=torch.int32, device="cuda")
+        got = w4.fp8_block_moe_gemm(q, s, xw, wsw, src, one, one * bm, 1, bm, out_dtype=FP32)
+        want, S = R.product(q[src[:4].long()], s[src[:4].long()], xw[1], wsw[1])
+        R.check_out(got[:4], want, S, R.blocks(K), FP32)
+        assert bool((got[4:] == 0).all())
+
+
+def test_two_streams_at_once(w4):
+    """Calls of both kernel forms that overlap on the GPU."""
+    g = _gen(17)
+    cases = []
+    for M, N, K in ((700, 4096, 1024), (8, 4096, 2048)):
+        x, xs = _matrix(g, M, K, row_block=1)
+        w, ws = _matrix(g, N, K, row_block=128)
+        cases.append((x, xs, w, ws, w4.fp8_block_gemm(x, xs, w, ws)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    outs = []
+    for i in range(24):
+        x, xs, w, ws, ref = cases[i % 2]
+        with torch.cuda.stream(streams[i % 4]):
+            outs.append((w4.fp8_block_gemm(x, xs, w, ws), ref))
+    torch.cuda.synchronize()
+    for out, ref in outs:
+        assert torch.equal(out, ref)
 
 
 # ------------------------------------------------------------------ together ----------------
