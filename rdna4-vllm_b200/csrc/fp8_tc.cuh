@@ -27,10 +27,9 @@ constexpr int kMaxSplit = 8;
 
 struct TcArgs {
     Fp8Args f;
-    int tile_rows;  // rows of x per tile
-    int split;      // CTAs per cluster
-    int n_tiles;    // weight tiles per row block
-    int out_vec;    // out's rows are 16-byte aligned
+    int split;    // CTAs per cluster
+    int n_tiles;  // weight tiles per row block
+    int out_vec;  // out's rows are 16-byte aligned
 };
 
 template <int N>

@@ -452,7 +452,6 @@ int launch_out(const TcArgs& t, bool wide, int64_t tiles, cudaStream_t st) {
 template <int NT>
 int launch_nt(TcArgs t, cudaStream_t st) {
     const Fp8Args& a = t.f;
-    t.tile_rows = NT;
     // row blocks that can hold work: with routing, at most one per slot
     int64_t blocks = (a.P + NT - 1) / NT;
     if (a.sorted_ids) blocks = std::min<int64_t>(blocks, a.num_slots);

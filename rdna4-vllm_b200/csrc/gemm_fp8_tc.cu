@@ -1,8 +1,9 @@
 // gemm_fp8_tc.cu — block-scaled FP8 products on the 5th-generation tensor cores.
 //
 // The kernel for blocks of more than 64 rows (fewer: gemm_fp8_swap.cu). A tile is 128 activation
-// rows (the MMA's M side: row = tensor-memory lane) times BN weight rows (its N side). Per 128-wide block g of K the tensor core returns acc = x_g w_g^T, and the
-// fold adds it to fp32 registers with one scalar per thread,
+// rows (the MMA's M side: row = tensor-memory lane) times BN weight rows (its N side). Per 128-wide
+// block g of K the tensor core returns acc = x_g w_g^T, and the fold adds it to fp32 registers with
+// one scalar per thread,
 //     tot[n] += (xs[row, g] * ws[n / 128, g]) * acc[n],
 // because a thread owns one row and the columns of one weight-scale block (two for the SiLU form,
 // gate and up).
@@ -329,84 +330,82 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 }
                 __syncwarp();
             } else if (copy_rows) {
-                // ---------------- gather warps: x rows in routing order, tall tiles ----------------
+                // ---------------- gather warps: x rows in routing order ----------------
                 // Lane l copies 16-byte chunk l % 8 of rows (l / 8) + 4 (warp index) + 8 i; a stage is
                 // announced when the next one has been requested, so that two are in flight.
-                if (copy_rows) {
-                    constexpr int kRowsPer = kRows / (4 * kGatherWarps);
-                    const int chunk = lane & 7, row0 = (warp - 2) * 4 + (lane >> 3);
-                    int pending = -1;  // stage requested but not announced
-                    auto announce = [&](int stage) {
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sm.full[stage]);
-                    };
-                    // the routing entries of the tile to enter next, fetched a tile ahead: lane l
-                    // holds this warp's rows l, l + 32, ...: row groups of 4 are dealt to the warps
-                    constexpr int kSlots = 4 / kGatherWarps;
-                    int slot[kSlots], e = -1;
-                    auto row_of = [&](int i) { return (i >> 2) * 4 * kGatherWarps + (warp - 2) * 4 + (i & 3); };
-                    auto look = [&](const Walk& w) {
-                        e = fetch_expert(w);
+                constexpr int kRowsPer = kRows / (4 * kGatherWarps);
+                const int chunk = lane & 7, row0 = (warp - 2) * 4 + (lane >> 3);
+                int pending = -1;  // stage requested but not announced
+                auto announce = [&](int stage) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.full[stage]);
+                };
+                // the routing entries of the tile to enter next, fetched a tile ahead: lane l
+                // holds this warp's rows l, l + 32, ...: row groups of 4 are dealt to the warps
+                constexpr int kSlots = 4 / kGatherWarps;
+                int slot[kSlots], e = -1;
+                auto row_of = [&](int i) { return (i >> 2) * 4 * kGatherWarps + (warp - 2) * 4 + (i & 3); };
+                auto look = [&](const Walk& w) {
+                    e = fetch_expert(w);
 #pragma unroll
-                        for (int i = 0; i < kSlots; ++i) {
-                            const int64_t r = (int64_t)w.rb * kRows + row_of(lane + 32 * i);
-                            slot[i] = fetch(r < rows ? a.sorted_ids + r : some_int);
-                        }
-                    };
-                    Walk w = cur;
-                    look(w);
-                    while (w.more()) {
-                        const bool present = expert(e) >= 0 && expert(e) < a.E;
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < kSlots; ++i)
-                            sm.src[row_of(lane + 32 * i)] =
-                                (int64_t)w.rb * kRows + row_of(lane + 32 * i) < rows && slot[i] >= 0 &&
-                                        slot[i] < a.num_slots
-                                    ? slot[i] / a.top_k
-                                    : -1;
-                        __syncwarp();
-                        int src[kRowsPer <= 16 ? kRowsPer : 1];  // or from shared memory each time
-                        if (kRowsPer <= 16)
-#pragma unroll
-                            for (int i = 0; i < kRowsPer; ++i)
-                                src[i % (kRowsPer <= 16 ? kRowsPer : 1)] = sm.src[row0 + i * 4 * kGatherWarps];
-                        w.next();
-                        if (!SPLIT) look(w);
-                        if (!present) {
-                            if (SPLIT) break;
-                            continue;
-                        }
-                        for (int g = g_lo; g < g_hi; ++g) {
-                            mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
-                            const int64_t k = (int64_t)g * kBlk + chunk * 16;
-                            const uint32_t xa = smem_u32(sm.ring[st.idx]);
-#pragma unroll
-                            for (int i = 0; i < kRowsPer; ++i) {
-                                const int tr = row0 + i * 4 * kGatherWarps;
-                                // absent rows and columns past K are written as zeros (source size 0)
-                                const int sr = kRowsPer <= 16 ? src[i % (kRowsPer <= 16 ? kRowsPer : 1)] : sm.src[tr];
-                                const bool ok = sr >= 0 && k < a.K;
-                                const uint8_t* p = a.x + (ok ? (int64_t)sr * a.K + k : 0);
-                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                                 xa + tr * 128 + ((chunk ^ (tr & 7)) << 4)),
-                                             "l"(p), "r"(ok ? 16 : 0)
-                                             : "memory");
-                            }
-                            asm volatile("cp.async.commit_group;" ::: "memory");
-                            if (pending >= 0) {
-                                asm volatile("cp.async.wait_group 1;" ::: "memory");
-                                announce(pending);
-                            }
-                            pending = (int)st.idx;
-                            st.next();
-                        }
-                        if (SPLIT) break;
+                    for (int i = 0; i < kSlots; ++i) {
+                        const int64_t r = (int64_t)w.rb * kRows + row_of(lane + 32 * i);
+                        slot[i] = fetch(r < rows ? a.sorted_ids + r : some_int);
                     }
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-                    if (pending >= 0) announce(pending);
+                };
+                Walk w = cur;
+                look(w);
+                while (w.more()) {
+                    const bool present = expert(e) >= 0 && expert(e) < a.E;
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < kSlots; ++i)
+                        sm.src[row_of(lane + 32 * i)] =
+                            (int64_t)w.rb * kRows + row_of(lane + 32 * i) < rows && slot[i] >= 0 &&
+                                    slot[i] < a.num_slots
+                                ? slot[i] / a.top_k
+                                : -1;
+                    __syncwarp();
+                    int src[kRowsPer <= 16 ? kRowsPer : 1];  // or from shared memory each time
+                    if (kRowsPer <= 16)
+#pragma unroll
+                        for (int i = 0; i < kRowsPer; ++i)
+                            src[i % (kRowsPer <= 16 ? kRowsPer : 1)] = sm.src[row0 + i * 4 * kGatherWarps];
+                    w.next();
+                    if (!SPLIT) look(w);
+                    if (!present) {
+                        if (SPLIT) break;
+                        continue;
+                    }
+                    for (int g = g_lo; g < g_hi; ++g) {
+                        mbar_wait(&sm.empty[st.idx], st.phase ^ 1, bad);
+                        const int64_t k = (int64_t)g * kBlk + chunk * 16;
+                        const uint32_t xa = smem_u32(sm.ring[st.idx]);
+#pragma unroll
+                        for (int i = 0; i < kRowsPer; ++i) {
+                            const int tr = row0 + i * 4 * kGatherWarps;
+                            // absent rows and columns past K are written as zeros (source size 0)
+                            const int sr = kRowsPer <= 16 ? src[i % (kRowsPer <= 16 ? kRowsPer : 1)] : sm.src[tr];
+                            const bool ok = sr >= 0 && k < a.K;
+                            const uint8_t* p = a.x + (ok ? (int64_t)sr * a.K + k : 0);
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                             xa + tr * 128 + ((chunk ^ (tr & 7)) << 4)),
+                                         "l"(p), "r"(ok ? 16 : 0)
+                                         : "memory");
+                        }
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        if (pending >= 0) {
+                            asm volatile("cp.async.wait_group 1;" ::: "memory");
+                            announce(pending);
+                        }
+                        pending = (int)st.idx;
+                        st.next();
+                    }
+                    if (SPLIT) break;
                 }
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                if (pending >= 0) announce(pending);
                 __syncwarp();
             }
             if (SPLIT) {
@@ -423,184 +422,180 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
             // ---------------- fold + epilogue ----------------
             const int q = warp & 3, fw = warp - kFoldWarp0, half = fw >> 2;
             const int row = q * 32 + lane;
-            {
-                // column of tot[j]: the plain form's half is contiguous; the SiLU form's holds 64
-                // gate columns, then the 64 matching up columns
-                auto col = [&](int j) {
-                    return SILU ? (j < 64 ? half * 64 + j : 128 + half * 64 + j - 64) : half * C::kCols + j;
-                };
-                const int64_t NB = (a.N + kBlk - 1) / kBlk;
-                int done = 0, turn = 0;  // turn: phase of the staging area
-                // Scales are fetched a block of K ahead, over the tiles' borders, routing entries a whole
-                // tile ahead. The fetches are unconditional, see fetch_expert.
-                const float *xs = a.xs, *ws0 = a.ws, *ws1 = a.ws;
-                bool present = false, dead = true;  // of the tile that enter() was given
-                int next_e = -1, next_slot = -1;    // of the tile to enter next
-                auto look = [&](const Walk& w) {
-                    const int64_t r = (int64_t)w.rb * kRows + row;
-                    next_e = fetch_expert(w);
-                    next_slot = fetch(a.sorted_ids && r < rows ? a.sorted_ids + r : some_int);
-                };
-                auto enter = [&](const Walk& w) {
-                    const int e = expert(next_e);
-                    const int64_t r = (int64_t)w.rb * kRows + row;
-                    present = w.more() && e >= 0 && e < a.E && g_lo < g_hi;
-                    int src = r < rows ? (a.sorted_ids ? next_slot : (int)r) : -1;
-                    if (a.sorted_ids) src = src >= 0 && src < a.num_slots ? src / a.top_k : -1;
-                    dead = !present || src < 0;
-                    const int64_t n0 = (int64_t)w.nt * n_step;
-                    const int64_t b0 = SILU ? n0 / kBlk : min((n0 + half * C::kCols) / kBlk, NB - 1);
-                    xs = a.xs + (dead ? 0 : src * (int64_t)G);
-                    ws0 = a.ws + (present ? (e * NB + b0) * G : 0);
-                    ws1 = SILU && present ? ws0 + (a.N / 2 / kBlk) * G : ws0;
-                };
-                float sx, s0, s1 = 0.f;
-                auto scales = [&](int g) {
-                    sx = fetch(xs + g);
-                    s0 = fetch(ws0 + g);
-                    if (SILU) s1 = fetch(ws1 + g);
-                };
-                Walk w = cur;
-                look(w);
-                enter(w);
-                scales(g_lo);
-                bool ready = false;  // the next accumulator was seen complete
-                while (w.more()) {
-                    const int64_t r0 = (int64_t)w.rb * kRows, r = r0 + row;
-                    const int64_t n0 = (int64_t)w.nt * n_step;
-                    const bool is_dead = dead, is_present = present;
-                    w.next();
-                    if (!SPLIT) look(w);
-                    float tot[C::kCols];
+            // column of tot[j]: the plain form's half is contiguous; the SiLU form's holds 64
+            // gate columns, then the 64 matching up columns
+            auto col = [&](int j) {
+                return SILU ? (j < 64 ? half * 64 + j : 128 + half * 64 + j - 64) : half * C::kCols + j;
+            };
+            const int64_t NB = (a.N + kBlk - 1) / kBlk;
+            int done = 0, turn = 0;  // turn: phase of the staging area
+            // Scales are fetched a block of K ahead, over the tiles' borders, routing entries a whole
+            // tile ahead. The fetches are unconditional, see fetch_expert.
+            const float *xs = a.xs, *ws0 = a.ws, *ws1 = a.ws;
+            bool present = false, dead = true;  // of the tile that enter() was given
+            int next_e = -1, next_slot = -1;    // of the tile to enter next
+            auto look = [&](const Walk& w) {
+                const int64_t r = (int64_t)w.rb * kRows + row;
+                next_e = fetch_expert(w);
+                next_slot = fetch(a.sorted_ids && r < rows ? a.sorted_ids + r : some_int);
+            };
+            auto enter = [&](const Walk& w) {
+                const int e = expert(next_e);
+                const int64_t r = (int64_t)w.rb * kRows + row;
+                present = w.more() && e >= 0 && e < a.E && g_lo < g_hi;
+                int src = r < rows ? (a.sorted_ids ? next_slot : (int)r) : -1;
+                if (a.sorted_ids) src = src >= 0 && src < a.num_slots ? src / a.top_k : -1;
+                dead = !present || src < 0;
+                const int64_t n0 = (int64_t)w.nt * n_step;
+                const int64_t b0 = SILU ? n0 / kBlk : min((n0 + half * C::kCols) / kBlk, NB - 1);
+                xs = a.xs + (dead ? 0 : src * (int64_t)G);
+                ws0 = a.ws + (present ? (e * NB + b0) * G : 0);
+                ws1 = SILU && present ? ws0 + (a.N / 2 / kBlk) * G : ws0;
+            };
+            float sx, s0, s1 = 0.f;
+            auto scales = [&](int g) {
+                sx = fetch(xs + g);
+                s0 = fetch(ws0 + g);
+                if (SILU) s1 = fetch(ws1 + g);
+            };
+            Walk w = cur;
+            look(w);
+            enter(w);
+            scales(g_lo);
+            bool ready = false;  // the next accumulator was seen complete
+            while (w.more()) {
+                const int64_t r0 = (int64_t)w.rb * kRows, r = r0 + row;
+                const int64_t n0 = (int64_t)w.nt * n_step;
+                const bool is_dead = dead, is_present = present;
+                w.next();
+                if (!SPLIT) look(w);
+                float tot[C::kCols];
 #pragma unroll
-                    for (int j = 0; j < C::kCols; ++j) tot[j] = 0.f;
-                    for (int g = is_present ? g_lo : g_hi; g < g_hi; ++g) {
-                        const float f0 = sx * s0, f1 = SILU ? sx * s1 : f0;
-                        int next_g = g + 1;
-                        if (next_g == g_hi) {
-                            next_g = g_lo;
-                            if (!SPLIT) enter(w);
-                        }
-                        scales(next_g);
-                        if (!ready) mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
+                for (int j = 0; j < C::kCols; ++j) tot[j] = 0.f;
+                for (int g = is_present ? g_lo : g_hi; g < g_hi; ++g) {
+                    const float f0 = sx * s0, f1 = SILU ? sx * s1 : f0;
+                    int next_g = g + 1;
+                    if (next_g == g_hi) {
+                        next_g = g_lo;
+                        if (!SPLIT) enter(w);
+                    }
+                    scales(next_g);
+                    if (!ready) mbar_wait(&sm.tfull[tb.idx], tb.phase, bad);
+                    __syncwarp();
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::);
+                    fold_block(tmem + ((uint32_t)(q * 32) << 16) + tb.idx * BN, col, f0, f1, tot, [&] {
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::);
                         __syncwarp();
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::);
-                        fold_block(tmem + ((uint32_t)(q * 32) << 16) + tb.idx * BN, col, f0, f1, tot, [&] {
-                            asm volatile("tcgen05.fence::before_thread_sync;" ::);
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&sm.tempty[tb.idx]);
-                            tb.next();
-                            ready = mbar_test(&sm.tfull[tb.idx], tb.phase);
-                        });
-                    }
-                    if (!is_present && !SPLIT) {
-                        enter(w);
-                        scales(g_lo);
-                    }
-                    // rows of zeros are zero whatever the lane's accumulator held: such a lane writes
-                    // `fill` over its staged row (a wait that gave up makes every row one, of NaN)
-                    const bool refill = is_dead || *bad;
-                    const float fill = *bad ? __int_as_float(0x7fffffff) : 0.f;
-                    if constexpr (SPLIT) {
-                        // park the partial tile; the ring is idle once the last accumulator was read
-                        if (row < kRows) {
-                            float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
-#pragma unroll
-                            for (int j = 0; j < C::kCols; j += 4)
-                                *reinterpret_cast<float4*>(part + col(j)) =
-                                    make_float4(tot[j], tot[j + 1], tot[j + 2], tot[j + 3]);
-                            if (refill)
-#pragma unroll 1
-                                for (int j = 0; j < C::kCols; ++j)
-                                    part[SILU ? (j & 63) + (j >> 6) * 128 + half * 64 : half * C::kCols + j] = fill;
-                        }
-                    } else if constexpr (SILU) {
-                        float m = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 64; j += 2) {
-                            silu_mul2(tot[j], tot[j + 1], tot[j + 64], tot[j + 65]);
-                            m = fmaxf(m, fmaxf(fabsf(tot[j]), fabsf(tot[j + 1])));
-                        }
-                        if (refill) m = fill;
-                        // the row's other 64 outputs are with the warp of the other half
-                        float(&amax)[2][kRows] = sm.amax[done & 1];
-                        amax[half][row] = m;
-                        asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
-                        m = fmaxf(m, amax[half ^ 1][row]);
-                        const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
-                        const float rcp = __frcp_rn(s);
-                        if (row < kRows && r < rows) {
-                            const int64_t inter = a.N / 2;
-                            if (half == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
-                            uint8_t* p = a.q + r * inter + n0 + half * 64;
-#pragma unroll
-                            for (int j = 0; j < 64; j += 32) {
-                                uint32_t u[8];
-#pragma unroll
-                                for (int i = 0; i < 8; ++i)
-                                    u[i] = quant4(tot[j + 4 * i], tot[j + 4 * i + 1], tot[j + 4 * i + 2],
-                                                  tot[j + 4 * i + 3], rcp);
-                                if (refill)
-#pragma unroll
-                                    for (int i = 0; i < 8; ++i) u[i] = fill == 0.f ? 0u : 0x7f7f7f7fu;
-                                store32(p + j, u);
-                            }
-                        }
-                    } else {
-                        const bool by_tma = tma_out((int)(r0 / kRows));
-                        const int64_t r_warp = r0 + q * 32;
-                        const int count = (int)min(rows - r_warp, (int64_t)32);
-                        constexpr int kPer = 16 / sizeof(Out);
-#pragma unroll
-                        for (int i = 0; i < kRounds; ++i) {
-                            uint8_t* so = sm.stage_out[half][0] + q * 4096;
-                            if (by_tma) {
-#pragma unroll
-                                for (int l = 0; l < C::kLines; ++l)
-                                    mbar_wait(&sm.ofree[half * C::kLines + l], turn ^ 1, bad);
-                            }
-#pragma unroll
-                            for (int l = 0; l < C::kLines; ++l)
-#pragma unroll
-                                for (int c = 0; c < 8; ++c) {
-                                    uint4 u;
-                                    const float* v = tot + (i * C::kLines + l) * kLineCols + c * kPer;
-                                    if constexpr (sizeof(Out) == 4)
-                                        u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
-                                                       __float_as_uint(v[2]), __float_as_uint(v[3]));
-                                    else
-                                        u = make_uint4(pack2<Out>(v[0], v[1]), pack2<Out>(v[2], v[3]),
-                                                       pack2<Out>(v[4], v[5]), pack2<Out>(v[6], v[7]));
-                                    *reinterpret_cast<uint4*>(so + l * (kRows * 128) + lane * 128 +
-                                                              ((c ^ (lane & 7)) << 4)) = u;
-                                }
-                            if (refill) {
-                                uint32_t v;
-                                if constexpr (sizeof(Out) == 4) v = __float_as_uint(fill);
-                                else v = pack2<Out>(fill, fill);
-#pragma unroll 1
-                                for (int c = 0; c < 8 * C::kLines; ++c)
-                                    *reinterpret_cast<uint4*>(so + (c >> 3) * (kRows * 128) + lane * 128 +
-                                                              (c & 7) * 16) = make_uint4(v, v, v, v);
-                            }
-                            if (by_tma) {
-                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                                __syncwarp();
-                                if (lane < C::kLines) mbar_arrive(&sm.ofull[half * C::kLines + lane]);
-                                turn ^= 1;
-                            } else {
-                                __syncwarp();
-                                for (int l = 0; l < C::kLines; ++l)
-                                    send_line<sizeof(Out)>(a, t.out_vec, so + l * (kRows * 128), r_warp, count,
-                                                           (int)n0 + half * C::kCols +
-                                                               (i * C::kLines + l) * kLineCols);
-                                __syncwarp();
-                            }
-                        }
-                    }
-                    ++done;
-                    if (SPLIT) break;
+                        if (lane == 0) mbar_arrive(&sm.tempty[tb.idx]);
+                        tb.next();
+                        ready = mbar_test(&sm.tfull[tb.idx], tb.phase);
+                    });
                 }
+                if (!is_present && !SPLIT) {
+                    enter(w);
+                    scales(g_lo);
+                }
+                // rows of zeros are zero whatever the lane's accumulator held: such a lane writes
+                // `fill` over its staged row (a wait that gave up makes every row one, of NaN)
+                const bool refill = is_dead || *bad;
+                const float fill = *bad ? __int_as_float(0x7fffffff) : 0.f;
+                if constexpr (SPLIT) {
+                    // park the partial tile; the ring is idle once the last accumulator was read
+                    if (row < kRows) {
+                        float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
+#pragma unroll
+                        for (int j = 0; j < C::kCols; j += 4)
+                            *reinterpret_cast<float4*>(part + col(j)) =
+                                make_float4(tot[j], tot[j + 1], tot[j + 2], tot[j + 3]);
+                        if (refill)
+#pragma unroll 1
+                            for (int j = 0; j < C::kCols; ++j)
+                                part[SILU ? (j & 63) + (j >> 6) * 128 + half * 64 : half * C::kCols + j] = fill;
+                    }
+                } else if constexpr (SILU) {
+                    float m = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 64; j += 2) {
+                        silu_mul2(tot[j], tot[j + 1], tot[j + 64], tot[j + 65]);
+                        m = fmaxf(m, fmaxf(fabsf(tot[j]), fabsf(tot[j + 1])));
+                    }
+                    if (refill) m = fill;
+                    // the row's other 64 outputs are with the warp of the other half
+                    float(&amax)[2][kRows] = sm.amax[done & 1];
+                    amax[half][row] = m;
+                    asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
+                    m = fmaxf(m, amax[half ^ 1][row]);
+                    const float s = __fdiv_rn(fmaxf(m, kAmaxFloor), kE4m3Max);
+                    const float rcp = __frcp_rn(s);
+                    if (r < rows) {
+                        const int64_t inter = a.N / 2;
+                        if (half == 0) a.qs[r * (inter / kBlk) + n0 / kBlk] = s;
+                        uint8_t* p = a.q + r * inter + n0 + half * 64;
+#pragma unroll
+                        for (int j = 0; j < 64; j += 32) {
+                            uint32_t u[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                u[i] = quant4(tot[j + 4 * i], tot[j + 4 * i + 1], tot[j + 4 * i + 2],
+                                              tot[j + 4 * i + 3], rcp);
+                            if (refill)
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) u[i] = fill == 0.f ? 0u : 0x7f7f7f7fu;
+                            store32(p + j, u);
+                        }
+                    }
+                } else {
+                    const bool by_tma = tma_out((int)(r0 / kRows));
+                    const int64_t r_warp = r0 + q * 32;
+                    const int count = (int)min(rows - r_warp, (int64_t)32);
+                    constexpr int kPer = 16 / sizeof(Out);
+#pragma unroll
+                    for (int i = 0; i < kRounds; ++i) {
+                        uint8_t* so = sm.stage_out[half][0] + q * 4096;
+#pragma unroll
+                        for (int l = 0; l < C::kLines; ++l)  // the last copy sent from it has read it
+                            mbar_wait(&sm.ofree[half * C::kLines + l], turn ^ 1, bad);
+#pragma unroll
+                        for (int l = 0; l < C::kLines; ++l)
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                uint4 u;
+                                const float* v = tot + (i * C::kLines + l) * kLineCols + c * kPer;
+                                if constexpr (sizeof(Out) == 4)
+                                    u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                                   __float_as_uint(v[2]), __float_as_uint(v[3]));
+                                else
+                                    u = make_uint4(pack2<Out>(v[0], v[1]), pack2<Out>(v[2], v[3]),
+                                                   pack2<Out>(v[4], v[5]), pack2<Out>(v[6], v[7]));
+                                *reinterpret_cast<uint4*>(so + l * (kRows * 128) + lane * 128 +
+                                                          ((c ^ (lane & 7)) << 4)) = u;
+                            }
+                        if (refill) {
+                            uint32_t v;
+                            if constexpr (sizeof(Out) == 4) v = __float_as_uint(fill);
+                            else v = pack2<Out>(fill, fill);
+#pragma unroll 1
+                            for (int c = 0; c < 8 * C::kLines; ++c)
+                                *reinterpret_cast<uint4*>(so + (c >> 3) * (kRows * 128) + lane * 128 +
+                                                          (c & 7) * 16) = make_uint4(v, v, v, v);
+                        }
+                        if (by_tma) {
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                            if (lane < C::kLines) mbar_arrive(&sm.ofull[half * C::kLines + lane]);
+                            turn ^= 1;
+                        } else {
+                            __syncwarp();
+                            for (int l = 0; l < C::kLines; ++l)
+                                send_line<sizeof(Out)>(a, t.out_vec, so + l * (kRows * 128), r_warp, count,
+                                                       (int)n0 + half * C::kCols +
+                                                           (i * C::kLines + l) * kLineCols);
+                            __syncwarp();
+                        }
+                    }
+                }
+                ++done;
+                if (SPLIT) break;
             }
             __syncwarp();
             if (SPLIT) {
@@ -677,7 +672,6 @@ int launch_fp8_tc(const Fp8Args& a, cudaStream_t st) {
         return launch_fp8_swap(a, st);
     TcArgs t{};
     t.f = a;
-    t.tile_rows = kRows;
     t.out_vec = out_vec(a);
     // row blocks that can hold work: with routing, at most one per slot and 128 rows of its block
     int64_t blocks = (a.P + kRows - 1) / kRows;
