@@ -198,7 +198,7 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
     if (warp == 0) {
         if (lane == 0) sm.bad = 0;
         if (lane < C::kStages) {
-            mbar_init(&sm.full[lane], copy_rows ? 1 + kGatherWarps : 1);
+            mbar_init(&sm.full[lane], copy_rows ? 1 + 32 * kGatherWarps : 1);
             mbar_init(&sm.empty[lane], 1);
         }
         if (lane < C::kAcc) {
@@ -274,6 +274,8 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                         if (!SPLIT) next_e = fetch_expert(w);
                         for (int g = e >= 0 && e < a.E ? g_lo : g_hi; g < g_hi; ++g) {
                             if (!full) mbar_wait(&sm.full[st.idx], st.phase, bad);
+                            // the copied rows were written by the generic proxy, the MMA reads by the other
+                            if (copy_rows) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                             if (!room) mbar_wait(&sm.tempty[tb.idx], tb.phase ^ 1, bad);
                             asm volatile("tcgen05.fence::after_thread_sync;" ::);
                             const uint32_t xa = smem_u32(sm.ring[st.idx]);
@@ -331,16 +333,10 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 __syncwarp();
             } else if (copy_rows) {
                 // ---------------- gather warps: x rows in routing order ----------------
-                // Lane l copies 16-byte chunk l % 8 of rows (l / 8) + 4 (warp index) + 8 i; a stage is
-                // announced when the next one has been requested, so that two are in flight.
+                // Lane l copies 16-byte chunk l % 8 of rows (l / 8) + 4 (warp index) + 8 i; the stage's
+                // barrier hears from each lane when its copies have arrived.
                 constexpr int kRowsPer = kRows / (4 * kGatherWarps);
                 const int chunk = lane & 7, row0 = (warp - 2) * 4 + (lane >> 3);
-                int pending = -1;  // stage requested but not announced
-                auto announce = [&](int stage) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.full[stage]);
-                };
                 // the routing entries of the tile to enter next, fetched a tile ahead: lane l
                 // holds this warp's rows l, l + 32, ...: row groups of 4 are dealt to the warps
                 constexpr int kSlots = 4 / kGatherWarps;
@@ -394,18 +390,14 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                                          "l"(p), "r"(ok ? 16 : 0)
                                          : "memory");
                         }
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        if (pending >= 0) {
-                            asm volatile("cp.async.wait_group 1;" ::: "memory");
-                            announce(pending);
-                        }
-                        pending = (int)st.idx;
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                                         smem_u32(&sm.full[st.idx]))
+                                     : "memory");
                         st.next();
                     }
                     if (SPLIT) break;
                 }
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                if (pending >= 0) announce(pending);
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
             }
             if (SPLIT) {
@@ -501,17 +493,15 @@ fp8_tc_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
                 const float fill = *bad ? __int_as_float(0x7fffffff) : 0.f;
                 if constexpr (SPLIT) {
                     // park the partial tile; the ring is idle once the last accumulator was read
-                    if (row < kRows) {
-                        float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
+                    float* part = reinterpret_cast<float*>(sm.ring) + row * C::kPitch;
 #pragma unroll
-                        for (int j = 0; j < C::kCols; j += 4)
-                            *reinterpret_cast<float4*>(part + col(j)) =
-                                make_float4(tot[j], tot[j + 1], tot[j + 2], tot[j + 3]);
-                        if (refill)
+                    for (int j = 0; j < C::kCols; j += 4)
+                        *reinterpret_cast<float4*>(part + col(j)) =
+                            make_float4(tot[j], tot[j + 1], tot[j + 2], tot[j + 3]);
+                    if (refill)
 #pragma unroll 1
-                            for (int j = 0; j < C::kCols; ++j)
-                                part[SILU ? (j & 63) + (j >> 6) * 128 + half * 64 : half * C::kCols + j] = fill;
-                    }
+                        for (int j = 0; j < C::kCols; ++j)
+                            part[SILU ? (j & 63) + (j >> 6) * 128 + half * 64 : half * C::kCols + j] = fill;
                 } else if constexpr (SILU) {
                     float m = 0.f;
 #pragma unroll
