@@ -18,6 +18,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "tcgen05.cuh"
 
 namespace w4a8 {
 
@@ -126,18 +127,22 @@ __device__ __forceinline__ float scale_of(float amax) {
     return isinf(a) ? a : quotient(a, kE4m3Max, 1.f / kE4m3Max);
 }
 
-// kSign: zeros keep their sign (the residual of a -0 is +0).
+// kSign: zeros keep their sign (the residual of a -0 is +0). The steps of `quotient`, two values an
+// instruction.
 template <bool kSign>
 __device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale) {
-    const float r = __frcp_rn(scale), s = isinf(scale) ? 0.f : scale;
-    float y[8];
+    const float r = __frcp_rn(scale), s = isinf(scale) ? 0.f : -scale;
+    const float2 r2 = make_float2(r, r), s2 = make_float2(s, s), none = make_float2(-0.f, -0.f);
+    uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        y[i] = quotient(v[i], s, r);
-        if (kSign) y[i] = copysignf(y[i], v[i]);
+    for (int i = 0; i < 8; i += 2) {
+        const float2 v2 = make_float2(v[i], v[i + 1]);
+        float2 y = ffma2(v2, r2, none);
+        y = ffma2(ffma2(y, s2, v2), r2, y);
+        if (kSign) y = make_float2(copysignf(y.x, v2.x), copysignf(y.y, v2.y));
+        u[i / 2] = f32x2_to_e4m3x2(y.x, y.y);
     }
-    return make_uint2((uint32_t)f32x2_to_e4m3x2(y[0], y[1]) | (uint32_t)f32x2_to_e4m3x2(y[2], y[3]) << 16,
-                      (uint32_t)f32x2_to_e4m3x2(y[4], y[5]) | (uint32_t)f32x2_to_e4m3x2(y[6], y[7]) << 16);
+    return make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
 }
 
 // 16 lanes quantise one block, 8 values each (zeros past the row's end).
@@ -150,41 +155,53 @@ __device__ __forceinline__ uint2 quant_block_half(const float (&v)[8], float& s)
     return quant8<kSign>(v, s);
 }
 
-// K % 8 == 0 and aligned rows: 16 lanes per block, kPerHalf blocks each, all requested first.
-// kFull: K % 128 == 0, where blocks follow one another in memory and need no row arithmetic.
-constexpr int kPerHalf = 4;
+// K % 8 == 0 and aligned rows: 8 lanes per block, 16 values each (what a block needs once, its
+// maximum over the lanes and its scale, costs as much as the 16 values), kPerLane blocks each, all
+// requested first. kFull: K % 128 == 0, where blocks follow one another in memory and need no row
+// arithmetic.
+constexpr int kPerLane = 2;
 template <typename T, bool kFull>
 __global__ void __launch_bounds__(256)
 act_quant_block_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                            float* __restrict__ scales, int64_t blocks, uint32_t K, uint32_t G) {
-    const int sub = threadIdx.x & 15;
-    const int64_t b0 = (int64_t)blockIdx.x * (16 * kPerHalf) + (threadIdx.x >> 4);
-    Vec8<T> x8[kPerHalf];
-    int64_t at[kPerHalf];
+    const int sub = threadIdx.x & 7;
+    const int64_t b0 = (int64_t)blockIdx.x * (32 * kPerLane) + (threadIdx.x >> 3);
+    Vec8<T> x8[kPerLane][2];
+    int64_t at[kPerLane];
+    bool ok[kPerLane][2];
 #pragma unroll
-    for (int i = 0; i < kPerHalf; ++i) {
-        const int64_t b = b0 + i * 16;
-        bool ok = b < blocks;
+    for (int i = 0; i < kPerLane; ++i) {
+        const int64_t b = b0 + i * 32;
+        uint32_t k = sub * 8;
         if (kFull) {
-            at[i] = (b0 * kBlk + sub * 8) + i * 16 * kBlk;
+            at[i] = (b0 * kBlk + sub * 8) + i * 32 * kBlk;
         } else {
             const int64_t r = blocks <= INT32_MAX ? (int64_t)((uint32_t)b / G) : b / G;
-            const uint32_t k = (uint32_t)(b - r * G) * kBlk + sub * 8;
+            k += (uint32_t)(b - r * G) * kBlk;
             at[i] = r * K + k;
-            ok = ok && k < K;
         }
-        x8[i].zero();
-        if (ok) x8[i].load(x + at[i]);
-        if (!kFull && !ok) at[i] = -1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            ok[i][h] = b < blocks && (kFull || k + h * 64 < K);
+            x8[i][h].zero();
+            if (ok[i][h]) x8[i][h].load(x + at[i] + h * 64);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < kPerHalf; ++i) {
-        const int64_t b = b0 + i * 16;
-        float v[8], s;
-        x8[i].get(v);
-        const uint2 u = quant_block_half<true>(v, s);
-        if (sub == 0 && b < blocks) scales[b] = s;
-        if (kFull ? b < blocks : at[i] >= 0) *reinterpret_cast<uint2*>(q + at[i]) = u;
+    for (int i = 0; i < kPerLane; ++i) {
+        float v[2][8];
+        float amax = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            x8[i][h].get(v[h]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[h][j]));
+        }
+        const float s = scale_of(lanes_max<8>(amax));
+        if (sub == 0 && b0 + i * 32 < blocks) scales[b0 + i * 32] = s;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (ok[i][h]) *reinterpret_cast<uint2*>(q + at[i] + h * 64) = quant8<true>(v[h], s);
     }
 }
 
@@ -358,7 +375,7 @@ template <typename T>
 int launch_quant(const void* x, int64_t M, int64_t K, uint8_t* q, float* scales, cudaStream_t st) {
     const int64_t G = (K + kBlk - 1) / kBlk, blocks = M * G;
     if (K % 8 == 0 && aligned(x, 16) && aligned(q, 8)) {
-        const int64_t ctas = (blocks + 16 * kPerHalf - 1) / (16 * kPerHalf);
+        const int64_t ctas = (blocks + 32 * kPerLane - 1) / (32 * kPerLane);
         if (ctas <= INT32_MAX) {
             if (K % kBlk == 0)
                 act_quant_block_vec_kernel<T, true><<<(unsigned)ctas, 256, 0, st>>>(
