@@ -93,6 +93,13 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
+// A kernel launched with kEarly (launch_persistent) may start before the stream's work ahead of it
+// is done; up to here it touches no memory, and from here on that work has ended.
+__device__ __forceinline__ void follow_launch() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -309,8 +316,9 @@ inline bool out_vec(const Fp8Args& a) {
     return start % 16 == 0;
 }
 
-// Persistent launch of `tiles` tiles over clusters of t.split CTAs.
-template <auto kKernel, typename... Maps>
+// Persistent launch of `tiles` tiles over clusters of t.split CTAs. kEarly: its set-up overlaps the
+// end of the stream's work ahead of it, and the next such launch's set-up the end of this one.
+template <auto kKernel, bool kEarly, typename... Maps>
 int launch_persistent(const TcArgs& t, int64_t tiles, size_t smem, cudaStream_t st, const Maps&... maps) {
     static std::atomic<bool> ready[kMaxDevices];  // this kernel's shared-memory limit is set
     const int dev = current_device();
@@ -325,11 +333,18 @@ int launch_persistent(const TcArgs& t, int64_t tiles, size_t smem, cudaStream_t 
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)t.split, 1, 1};
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (kEarly) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (t.split > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n++].val.clusterDim = {(unsigned)t.split, 1, 1};
+    }
     cfg.attrs = at;
-    cfg.numAttrs = t.split > 1 ? 1 : 0;
+    cfg.numAttrs = n;
     e = cudaLaunchKernelEx(&cfg, kKernel, t, maps...);
     return e != cudaSuccess ? (int)e : launch_status();
 }

@@ -21,11 +21,12 @@
 // every CTA parks its part of it there (distributed shared memory), and after a cluster barrier the
 // owner adds the parts in rank order.
 //
-// Measured: gate_up of 32 tokens over 256 experts (2048 -> 2 x 512, 346 MB) 61 us, 87 % of the
-// measured copy bandwidth; down of the same (174 MB) 34.8 us, 78 %: its tiles have four blocks of K,
-// so scales are fetched for a new tile every other microsecond, behind the weights in the queue.
-// Dense batches of up to 128 rows take 5 to 8 us on the device, most of it latency: set-up 0.7,
-// first data 0.9, the cluster's join 0.4.
+// Measured: gate_up of 32 tokens over 256 experts (2048 -> 2 x 512, 346 MB) 61 us, 88 % of the
+// measured copy bandwidth; down of the same (174 MB) 32.9 us, 82 %: 8.8 tiles a CTA run as 9, and
+// padding rows are written too. Dense batches of up to 128 rows take 4 to 8 us on the device, most of
+// it latency: set-up 0.7, first data 0.9, the cluster's join 0.4. The set-up overlaps the end of the
+// work ahead in the stream (kEarly); without that, 1 x 4096 x 2048 took 8.0 us a call instead of 6.7,
+// 128 x 2048 x 4096 10.2 instead of 7.6, down 34.6.
 //
 // Waits are bounded as in gemm_fp8_tc.cu: one that gives up leaves NaN in the tile's outputs.
 #include "fp8_tc.cuh"
@@ -107,12 +108,9 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
 
     const int S = SPLIT ? t.split : 1;
     const int rank = SPLIT ? (int)cluster_rank() : 0;
-    const int64_t rows = a.ntp ? max((int64_t)0, min((int64_t)a.ntp[0], a.P)) : a.P;
-    const int blocks = (int)((rows + NT - 1) / NT);
     const int G = (int)a.G;
     const int g_lo = (int)((int64_t)G * rank / S), g_hi = (int)((int64_t)G * (rank + 1) / S);
     const int n_step = SILU ? 128 : WR;  // outputs per tile
-    const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
     auto expert_of = [&](int rb) { return a.expert_ids ? fetch(a.expert_ids + rb) : 0; };
 
     if (tid == 32 * 2) {
@@ -151,6 +149,10 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         asm volatile("bar.sync 8, %0;" ::"n"(kThreads) : "memory");
         asm volatile("tcgen05.fence::after_thread_sync;" ::);
     }
+    follow_launch();
+    const int64_t rows = a.ntp ? max((int64_t)0, min((int64_t)a.ntp[0], a.P)) : a.P;
+    const int blocks = (int)((rows + NT - 1) / NT);
+    const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
     if (SPLIT) cluster_arrive();  // awaited before the first part is parked with another CTA
 
     // One pass runs all of the CTA's tiles; with a split it is one tile, and the cluster meets
@@ -439,8 +441,8 @@ int launch_t(const TcArgs& t, int64_t tiles, cudaStream_t st) {
     CUtensorMap tmx, tmw;
     if (!make_maps(t.f, t.f.sorted_ids ? 1 : NT, WR, &tmx, &tmw))
         return set_error("fp8_block: tensor map encoding failed");
-    return launch_persistent<fp8_swap_kernel<NT, WR, Out, SPLIT>>(t, tiles, sizeof(Smem<NT, WR>) + 1024,
-                                                                  st, tmx, tmw);
+    return launch_persistent<fp8_swap_kernel<NT, WR, Out, SPLIT>, true>(
+        t, tiles, sizeof(Smem<NT, WR>) + 1024, st, tmx, tmw);
 }
 
 template <int NT, typename Out>

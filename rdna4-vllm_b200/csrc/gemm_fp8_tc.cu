@@ -634,8 +634,8 @@ int launch_t(TcArgs t, int64_t tiles, cudaStream_t st) {
     if (kStaged && t.out_vec &&
         !make_tma_map_u8(&tmo, a.out, (uint64_t)a.P, (uint64_t)pitch, 128, kRows, CU_TENSOR_MAP_SWIZZLE_128B))
         return set_error("fp8_block: tensor map encoding failed");
-    return launch_persistent<fp8_tc_kernel<BN, Out, SPLIT>>(t, tiles, sizeof(Smem<BN, kStaged>) + 1024,
-                                                            st, tmx, tmw, tmo);
+    return launch_persistent<fp8_tc_kernel<BN, Out, SPLIT>, false>(
+        t, tiles, sizeof(Smem<BN, kStaged>) + 1024, st, tmx, tmw, tmo);
 }
 
 template <typename Out>
