@@ -24,12 +24,15 @@
 // sums rows r, r + S, ... over the cluster in rank order (distributed shared memory), so the
 // result does not depend on timing.
 //
-// What bounds it. A block of a 128 x 256 tile is 512 cycles of MMA, but its 48 KB come from L2 at 57
-// to 64 bytes a cycle and SM, 770 to 840 cycles however little is computed on them, and long runs
-// sit at the 1000 W power cap (1.6 to 1.7 GHz). 8192 x 8192 x 2048 takes 159 us, 1.73 PFLOP/s;
-// gate_up of 4096 tokens over 256 experts (2048 -> 2 x 512) 153 us, down of the same 94. A pair of CTAs on a tile of 256 x 256 (cta_group::2,
-// 32 KB a block) was slower, 197 us against 173 for the first at that point: with a fold after every
-// block only two accumulators fit, and the way from MMA to both CTAs' folds and back is 2400 cycles.
+// What bounds it: the 1000 W power cap, which takes the clock to 1.6 GHz and below in long runs.
+// 8192 x 8192 x 2048 takes 160 us, 1.72 PFLOP/s; gate_up of 4096 tokens over 256 experts (2048 -> 2 x
+// 512) 151 us, down of the same 94.5. In cycles a block of a 128 x 256 tile takes 930: MMA 590, to
+// the fold and back 570, fold 400, over two accumulators, while its 48 KB come from L2 in 770 to 840.
+// Waits that poll rather than suspend make the way shorter and the runs 3 % longer. A pair of CTAs on
+// a tile of 256 x 256 (cta_group::2, 32 KB a block) was slower, 197 us against 173 for the first at
+// that point: with a fold after every block only two accumulators fit, and the way from MMA to both
+// CTAs' folds and back is 2400 cycles. Two MMAs of 128 columns with barriers of their own read x twice
+// from shared memory: 168 us.
 //
 // Every mbarrier wait is bounded (sm100.cuh). When one gives up, the CTA stops waiting, waits
 // (boundedly) for its own copies in flight, writes NaN to the tile's outputs and frees tensor
