@@ -521,6 +521,63 @@ def test_side_stream_and_graphs(w4):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("T,E,k,H,I", [(8, 4, 2, 512, 256), (32, 16, 4, 1024, 512), (24, 64, 8, 2048, 128)])
+def test_launches_that_follow_one_another(w4, T, E, k, H, I):
+    """Chains in which each call reads what the one before wrote, into the same buffers every time and
+    without a wait between, eager and captured, against the same calls waited for one by one."""
+    g = _gen(T + E)
+    w1, w2, s1, s2 = _layer(g, T, E, H, I)
+    w3, s3 = w2[0].view(torch.uint8).repeat(1, 2), s2[0].repeat(1, 2)
+    bm = 16
+    inputs = []
+    for i in range(6):
+        q, sc = _matrix(g, T, H, row_block=1)
+        inputs.append((q, sc) + _routing(T, E, k, bm, i + 2))
+    size = max(t[2].numel() for t in inputs)
+    s = torch.empty(size, dtype=torch.int32, device="cuda")
+    e = torch.empty(size // bm, dtype=torch.int32, device="cuda")
+    x, xs, n = inputs[0][0].clone(), inputs[0][1].clone(), inputs[0][4].clone()
+
+    def load(i):
+        q, sc, si, ei, ni = inputs[i]
+        x.copy_(q), xs.copy_(sc), n.copy_(ni)
+        s.fill_(T * k), e.fill_(-1)
+        s[:si.numel()].copy_(si), e[:ei.numel()].copy_(ei)
+
+    def chain(wait=lambda: None):
+        h, hs = w4.fp8_block_moe_gemm1_silu(x, xs, w1, s1, s, e, n, k, bm)
+        wait()
+        y = w4.fp8_block_moe_gemm(h, hs, w2, s2, None, e, n, 1, bm, BF16)
+        wait()
+        a, b = w4.act_quant_fp8_block(y[:T])  # the first rows: below every count here
+        wait()
+        z = w4.fp8_block_gemm(a, b, w1[0], s1[0], BF16)
+        wait()
+        a, b = w4.act_quant_fp8_block(z)
+        wait()
+        return w4.fp8_block_gemm(a, b, w3, s3, FP32)
+
+    assert all(int(t[4]) >= T for t in inputs)
+    want = []
+    for i in range(6):
+        load(i)
+        want.append(chain(torch.cuda.synchronize))
+        torch.cuda.synchronize()
+    got = []
+    for i in [0, 1, 2, 3, 4, 5] * 8:
+        load(i)
+        got.append((i, chain()))
+    for i, z in got:
+        assert torch.equal(z, want[i])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        z = chain()
+    for i in [3, 0, 5, 1, 4, 2] * 4:
+        load(i)
+        graph.replay()
+        assert torch.equal(z, want[i])
+
+
 def test_refusals(w4):
     x = torch.zeros(16, 256, dtype=torch.uint8, device="cuda")
     xs = torch.zeros(16, 2, device="cuda")
