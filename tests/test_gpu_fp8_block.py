@@ -578,6 +578,39 @@ def test_launches_that_follow_one_another(w4, T, E, k, H, I):
         assert torch.equal(z, want[i])
 
 
+def test_capture_with_a_fork(w4):
+    """Two captured branches that join in front of a third product; outputs of both are read."""
+    g = _gen(5)
+    x1, s1 = _matrix(g, 16, 512, row_block=1)
+    x2, s2 = _matrix(g, 16, 512, row_block=1)
+    w, ws = _matrix(g, 512, 512, row_block=128)
+
+    def joined(fork):
+        main = torch.cuda.current_stream()
+        side = torch.cuda.Stream() if fork else main
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b, bs = w4.act_quant_fp8_block(w4.fp8_block_gemm(x2, s2, w, ws))
+            b = w4.fp8_block_gemm(b, bs, w, ws, FP32)
+        a, as_ = w4.act_quant_fp8_block(w4.fp8_block_gemm(x1, s1, w, ws))
+        z = w4.fp8_block_gemm(a, as_, w, ws, FP32)
+        main.wait_stream(side)
+        q, s = w4.act_quant_fp8_block(z + b)
+        return w4.fp8_block_gemm(q, s, w, ws), w4.fp8_block_gemm(x2, s2, w, ws), b
+
+    want = [t.clone() for t in joined(False)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = joined(True)
+    for _ in range(20):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 def test_refusals(w4):
     x = torch.zeros(16, 256, dtype=torch.uint8, device="cuda")
     xs = torch.zeros(16, 2, device="cuda")
