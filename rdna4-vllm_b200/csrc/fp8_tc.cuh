@@ -76,14 +76,6 @@ __device__ __forceinline__ void prefetch_l2(const void* p) {
     asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
-// x's row of output row r, or -1 when r is a row of zeros (absent expert e, padding slot).
-__device__ __forceinline__ int64_t source_row(const Fp8Args& a, int64_t r, int64_t rows, int e) {
-    if (r >= rows || e < 0 || e >= a.E) return -1;
-    if (!a.sorted_ids) return r;
-    const int slot = a.sorted_ids[r];
-    return slot >= 0 && slot < a.num_slots ? slot / a.top_k : -1;
-}
-
 // True in one lane of a converged warp. The copies, MMAs and commits take uniform operands, and
 // behind this condition the compiler need not serialise the lanes to make them so (a comparison
 // of the lane number cost 200 cycles for each).
