@@ -11,7 +11,6 @@ True calls this package's operators.
 """
 from __future__ import annotations
 
-import functools
 import os
 import sys
 
@@ -202,7 +201,6 @@ def prepare(case, seed):
 
 # ---- one pass ------------------------------------------------------------------------------
 
-@functools.cache
 def _package():
     at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rdna4-vllm_b200")
     if at not in sys.path:
