@@ -35,12 +35,13 @@ __global__ void build_inverse_map_kernel(const int32_t* __restrict__ sorted_ids,
 }
 
 // One CTA per (token, 512-channel chunk); each thread reduces 2 adjacent channels. Generic
-// path for N % 8 != 0 or unaligned rows.
+// path for N % 8 != 0 or unaligned rows. `pairs`: every row starts on a 4-byte boundary (N even, and
+// out2 itself: a view may start at any element), so that two channels are one load.
 template <typename InT, typename OutT>
 __global__ void __launch_bounds__(256)
 gather_reduce_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
                      const float* __restrict__ topk_w, OutT* __restrict__ out, int64_t N,
-                     int top_k) {
+                     int top_k, bool pairs) {
     const int64_t t = blockIdx.y;
     const int64_t n = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 2;
     if (n >= N) return;
@@ -51,7 +52,7 @@ gather_reduce_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ s
         if (r < 0) continue;
         const float w = topk_w[t * top_k + j];
         const InT* rowp = out2 + (int64_t)r * N + n;
-        if (pair && (N % 2 == 0)) {
+        if (pairs) {  // N is even: n + 1 < N
             const float2 v = pair_f32<InT>(*reinterpret_cast<const uint32_t*>(rowp));
             a0 = __fadd_rn(a0, __fmul_rn(w, v.x));
             a1 = __fadd_rn(a1, __fmul_rn(w, v.y));
@@ -135,8 +136,9 @@ static int launch_reduce(const InT* out2, const int32_t* slot_to_row, const floa
                                                                       out, N, top_k);
     } else {
         const dim3 grid((unsigned)((N + 511) / 512), (unsigned)M);
+        const bool pairs = N % 2 == 0 && (reinterpret_cast<uintptr_t>(out2) & 3) == 0;
         gather_reduce_kernel<InT, OutT><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w, out,
-                                                                  N, top_k);
+                                                                  N, top_k, pairs);
     }
     return launch_status();
 }
