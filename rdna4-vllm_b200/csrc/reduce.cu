@@ -34,17 +34,22 @@ __global__ void build_inverse_map_kernel(const int32_t* __restrict__ sorted_ids,
     if (slot >= 0 && slot < num_slots) slot_to_row[slot] = (int32_t)r;
 }
 
+// The token of a CTA: tokens lie over y and z of the grid, since y alone ends at 65535.
+__device__ __forceinline__ int64_t grid_token() {
+    return (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
+}
+
 // One CTA per (token, 512-channel chunk); each thread reduces 2 adjacent channels. Generic
 // path for N % 8 != 0 or unaligned rows. `pairs`: every row starts on a 4-byte boundary (N even, and
 // out2 itself: a view may start at any element), so that two channels are one load.
 template <typename InT, typename OutT>
 __global__ void __launch_bounds__(256)
 gather_reduce_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
-                     const float* __restrict__ topk_w, OutT* __restrict__ out, int64_t N,
-                     int top_k, bool pairs) {
-    const int64_t t = blockIdx.y;
+                     const float* __restrict__ topk_w, OutT* __restrict__ out, int64_t M,
+                     int64_t N, int top_k, bool pairs) {
+    const int64_t t = grid_token();
     const int64_t n = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 2;
-    if (n >= N) return;
+    if (t >= M || n >= N) return;
     float a0 = 0.f, a1 = 0.f;
     const bool pair = (n + 1 < N);
     for (int j = 0; j < top_k; ++j) {
@@ -72,11 +77,12 @@ constexpr int kMaxTopK = 16;
 template <typename InT, typename OutT>
 __global__ void __launch_bounds__(256)
 gather_reduce_vec_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
-                         const float* __restrict__ topk_w, OutT* __restrict__ out, int64_t N,
-                         int top_k) {
+                         const float* __restrict__ topk_w, OutT* __restrict__ out, int64_t M,
+                         int64_t N, int top_k) {
     __shared__ int32_t rows[kMaxTopK];
     __shared__ float wts[kMaxTopK];
-    const int64_t t = blockIdx.y;
+    const int64_t t = grid_token();
+    if (t >= M) return;
     if (threadIdx.x < top_k) {
         rows[threadIdx.x] = slot_to_row[t * top_k + threadIdx.x];
         wts[threadIdx.x] = topk_w[t * top_k + threadIdx.x];
@@ -130,15 +136,17 @@ static int launch_reduce(const InT* out2, const int32_t* slot_to_row, const floa
     const bool vec = N % 8 == 0 && top_k <= kMaxTopK &&
                      (reinterpret_cast<uintptr_t>(out2) & 15) == 0 &&
                      (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    const int64_t z = (M + 65534) / 65535;
+    const unsigned y = (unsigned)((M + z - 1) / z);
     if (vec) {
-        const dim3 grid((unsigned)((N / 8 + 255) / 256), (unsigned)M);
+        const dim3 grid((unsigned)((N / 8 + 255) / 256), y, (unsigned)z);
         gather_reduce_vec_kernel<InT, OutT><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w,
-                                                                      out, N, top_k);
+                                                                      out, M, N, top_k);
     } else {
-        const dim3 grid((unsigned)((N + 511) / 512), (unsigned)M);
         const bool pairs = N % 2 == 0 && (reinterpret_cast<uintptr_t>(out2) & 3) == 0;
+        const dim3 grid((unsigned)((N + 511) / 512), y, (unsigned)z);
         gather_reduce_kernel<InT, OutT><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w, out,
-                                                                  N, top_k, pairs);
+                                                                  M, N, top_k, pairs);
     }
     return launch_status();
 }

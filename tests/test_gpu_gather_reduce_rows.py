@@ -47,3 +47,11 @@ def test_views_off_their_alignment(w4, N, off, dtype):
     got = w4.mmq_fp8_moe_gather_reduce(view, s, tw, n, 3)
     assert torch.equal(got, w4.mmq_fp8_moe_gather_reduce(rows, s, tw, n, 3))
     assert torch.equal(got, _expected(rows, s, tw, 3))
+
+
+@pytest.mark.parametrize("M,N,top_k", [(65535, 8, 1), (65536, 8, 1), (70000, 16, 2), (70000, 6, 2),
+                                       (140000, 8, 3), (140001, 5, 1)])
+def test_more_tokens_than_a_grid_dimension_holds(w4, M, N, top_k):
+    """Above 65535 tokens, through the vectorised kernel (N a multiple of 8) and the generic one."""
+    rows, s, n, tw = _case(M, N, top_k, FP16, M + N)
+    assert torch.equal(w4.mmq_fp8_moe_gather_reduce(rows, s, tw, n, top_k), _expected(rows, s, tw, top_k))
