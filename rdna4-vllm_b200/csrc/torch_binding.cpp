@@ -228,11 +228,16 @@ at::Tensor mmq_fp8_moe_gather_reduce_forward(const at::Tensor& out2,
     const bool bf16 = out2.scalar_type() == at::kBFloat16;
     TORCH_CHECK(out2.is_cuda() && (bf16 || out2.scalar_type() == at::kHalf) && out2.dim() == 2,
                 "out2 must be (P,N) fp16 or bf16 CUDA");
-    TORCH_CHECK(sorted_token_ids.scalar_type() == at::kInt && ntp.scalar_type() == at::kInt,
-                "sorted_token_ids / num_tokens_post_padded must be int32");
+    TORCH_CHECK(sorted_token_ids.scalar_type() == at::kInt && ntp.scalar_type() == at::kInt &&
+                    sorted_token_ids.dim() == 1 && ntp.numel() >= 1,
+                "sorted_token_ids (P,) / num_tokens_post_padded (1,) must be int32");
     TORCH_CHECK(topk_weights.scalar_type() == at::kFloat, "topk_weights must be fp32");
-    TORCH_CHECK(out2.is_contiguous() && topk_weights.is_contiguous(),
-                "out2 and topk_weights must be contiguous");
+    TORCH_CHECK(sorted_token_ids.device() == out2.device() && ntp.device() == out2.device() &&
+                    topk_weights.device() == out2.device(),
+                "sorted_token_ids, topk_weights and num_tokens_post_padded must be on out2's device");
+    TORCH_CHECK(out2.is_contiguous() && topk_weights.is_contiguous() &&
+                    sorted_token_ids.is_contiguous(),
+                "out2, sorted_token_ids and topk_weights must be contiguous");
     TORCH_CHECK(top_k > 0 && topk_weights.numel() % top_k == 0,
                 "topk_weights.numel() must be M*top_k");
     TORCH_CHECK(sorted_token_ids.size(0) <= out2.size(0),

@@ -55,3 +55,31 @@ def test_more_tokens_than_a_grid_dimension_holds(w4, M, N, top_k):
     """Above 65535 tokens, through the vectorised kernel (N a multiple of 8) and the generic one."""
     rows, s, n, tw = _case(M, N, top_k, FP16, M + N)
     assert torch.equal(w4.mmq_fp8_moe_gather_reduce(rows, s, tw, n, top_k), _expected(rows, s, tw, top_k))
+
+
+def test_refusals(w4):
+    """Operands that the kernel could not read, or would read in another order."""
+    rows, s, n, tw = _case(4, 16, 2, FP16, 1)
+    twice = s.repeat_interleave(2)
+    bad = [(rows, s.cpu(), tw, n), (rows, s, tw.cpu(), n), (rows, s, tw, n.cpu()), (rows, twice[::2], tw, n),
+           (rows, s.reshape(2, 4), tw, n), (rows, s, tw, n[:0]), (rows, s.long(), tw, n),
+           (rows, s, tw.half(), n), (rows.t(), s, tw, n), (rows, twice, tw, n), (rows.int(), s, tw, n)]
+    for args in bad:
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            w4.mmq_fp8_moe_gather_reduce(*args, 2)
+    assert torch.equal(w4.mmq_fp8_moe_gather_reduce(rows, s, tw, n, 2), _expected(rows, s, tw, 2))
+
+
+def test_layer_refuses_weights_of_another_device(w4):
+    from w4a8_fp8_wmma.fp8_block import run_fp8_block_moe
+    x = torch.ones(2, 128, dtype=BF16, device="cuda")
+    w1 = torch.zeros(2, 256, 128, dtype=torch.uint8, device="cuda")
+    w2 = torch.zeros(2, 128, 128, dtype=torch.uint8, device="cuda")
+    s1, s2 = torch.ones(2, 2, 1, device="cuda"), torch.ones(2, 1, 1, device="cuda")
+    ids = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    tw = torch.ones(2, 1, device="cuda")
+    assert bool((run_fp8_block_moe(x, w1, w2, s1, s2, tw, ids) == 0).all())
+    assert bool((run_fp8_block_moe(x, w1, w2, s1, s2, tw, ids.long()) == 0).all())  # converted on the way
+    for change in (dict(topk_weights=tw.cpu()), dict(topk_ids=ids.cpu())):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            run_fp8_block_moe(x, w1, w2, s1, s2, **{"topk_weights": tw, "topk_ids": ids, **change})
