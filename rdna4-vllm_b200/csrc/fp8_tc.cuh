@@ -61,15 +61,16 @@ struct Walk {
 };
 
 // A load that stays where it is written: fetched a tile ahead of its use, it would otherwise be
-// moved down to it to save a register.
+// moved down to it to save a register. Not on the read-only path (ld.global.nc): in a kernel that
+// starts early (launch_persistent) the work ahead may write this memory while the kernel is there.
 __device__ __forceinline__ float fetch(const float* p) {
     float v;
-    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
     return v;
 }
 __device__ __forceinline__ int fetch(const int32_t* p) {
     int v;
-    asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
     return v;
 }
 __device__ __forceinline__ void prefetch_l2(const void* p) {

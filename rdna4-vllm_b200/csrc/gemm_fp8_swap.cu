@@ -150,7 +150,7 @@ fp8_swap_kernel(const TcArgs t, const __grid_constant__ CUtensorMap tmx,
         asm volatile("tcgen05.fence::after_thread_sync;" ::);
     }
     follow_launch();
-    const int64_t rows = a.ntp ? max((int64_t)0, min((int64_t)a.ntp[0], a.P)) : a.P;
+    const int64_t rows = a.ntp ? max((int64_t)0, min((int64_t)fetch(a.ntp), a.P)) : a.P;
     const int blocks = (int)((rows + NT - 1) / NT);
     const Walk first(blockIdx.x / S, gridDim.x / S, t.n_tiles, blocks);
     if (SPLIT) cluster_arrive();  // awaited before the first part is parked with another CTA
