@@ -160,16 +160,29 @@ __device__ __forceinline__ float4 ld_cluster(const float* p, uint32_t rank) {
     return v;
 }
 
-// silu(g) * u of two outputs, g0 and u0 replaced by the results. One reciprocal serves both
-// denominators d = 1 + exp(-g), 1 / d0 = d1 / (d0 d1): the special-function unit, at 16 a cycle
-// and SM, is what this step waits for. exp(-g) is cut at 2^62 to keep the product in range (silu
-// is below 2^-56 there). Together within 12 units of 2^-24, plus |g| 2^-24 from the exponential's
-// argument: below the product sums' own error.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+
+// silu(g) * u of two outputs, g0 and u0 replaced by the results. With e = exp(-|g|), which cannot
+// overflow, silu(g) is g / (1 + e) for g >= 0 and g e / (1 + e) below, and u comes last. One reciprocal
+// serves both denominators d = 1 + e in (1, 2], 1 / d0 = d1 / (d0 d1): the special-function unit, at 16
+// a cycle and SM, is what this step waits for. A NaN's d is cut to 2, so that its neighbour keeps its
+// value. Together within 16 units of 2^-24, plus 1.25 |g| of them for g < 0 from the exponential's
+// argument; below -87 e is subnormal, each of e and silu within 2^-149, and from -104 on it is 0.
 __device__ __forceinline__ void silu_mul2(float& g0, float& g1, float u0, float u1) {
-    const float d0 = 1.f + fminf(__expf(-g0), 0x1p62f), d1 = 1.f + fminf(__expf(-g1), 0x1p62f);
-    const float r = __fdividef(1.f, d0 * d1);
-    g0 = g0 * u0 * (d1 * r);
-    g1 = g1 * u1 * (d0 * r);
+    const float e0 = __expf(-fabsf(g0)), e1 = __expf(-fabsf(g1));
+    const float d0 = 1.f + fminf(e0, 1.f), d1 = 1.f + fminf(e1, 1.f);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
+    const float2 g = make_float2(g0 >= 0.f ? g0 : g0 * e0, g1 >= 0.f ? g1 : g1 * e1);
+    const float2 h = mul2(mul2(g, mul2(make_float2(d1, d0), make_float2(r, r))), make_float2(u0, u1));
+    g0 = h.x;
+    g1 = h.y;
 }
 
 // Four e4m3 bytes of v / scale, rcp = 1 / scale. The values carry more than the 2^-23 by which the

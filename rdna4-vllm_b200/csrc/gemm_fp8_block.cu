@@ -87,8 +87,10 @@ __global__ void __launch_bounds__(256) fp8_simple_kernel(const Fp8Args a) {
             float amax = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float gate = tot[j];
-                tot[j] = src >= 0 ? gate / (1.f + expf(-gate)) * tot[(j + 8) % (kNw / 16)] : 0.f;
+                // silu by exp(-|gate|), which does not overflow (fp8_tc.cuh: silu_mul2)
+                const float gate = tot[j], e = expf(-fabsf(gate));
+                const float silu = (gate >= 0.f ? gate : gate * e) / (1.f + e);
+                tot[j] = src >= 0 ? silu * tot[(j + 8) % (kNw / 16)] : 0.f;
                 amax = fmaxf(amax, fabsf(tot[j]));
             }
 #pragma unroll
