@@ -197,6 +197,11 @@ W4A8_API int w4a8_moe_gather_reduce_bf16(const void* out2, const int32_t* sorted
                                 const float* topk_weights, const int32_t* num_tokens_post_padded,
                                 float* out, int64_t M, int64_t N, int64_t P, int64_t top_k,
                                 void* workspace, size_t workspace_bytes, w4a8_stream_t stream);
+/* The same with fp32 rows (that product for an fp32 result). */
+W4A8_API int w4a8_moe_gather_reduce_f32(const void* out2, const int32_t* sorted_token_ids,
+                               const float* topk_weights, const int32_t* num_tokens_post_padded,
+                               float* out, int64_t M, int64_t N, int64_t P, int64_t top_k,
+                               void* workspace, size_t workspace_bytes, w4a8_stream_t stream);
 
 /*
  * silu_and_mul on fp16 rows: x (M, 2*inter) [gate | up] -> out (M, inter),

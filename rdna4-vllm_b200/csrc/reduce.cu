@@ -16,13 +16,30 @@ namespace w4a8 {
 
 namespace {
 
-// Row element types: fp16, or bf16 (the rows of a bf16 model's block-scaled down product).
+// Row element types: fp16, or the rows of a block-scaled down product, bf16 for a bf16 model and
+// fp32 for an fp32 result.
+__device__ __forceinline__ float row_f32(float v) { return v; }
 __device__ __forceinline__ float row_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float row_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename InT>
 __device__ __forceinline__ float2 pair_f32(uint32_t w) {
     const InT* h = reinterpret_cast<const InT*>(&w);
     return make_float2(row_f32(h[0]), row_f32(h[1]));
+}
+// The values of 16 bytes of a row.
+template <typename InT>
+__device__ __forceinline__ void unpack16(uint4 v, float (&f)[16 / sizeof(InT)]) {
+    const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if constexpr (sizeof(InT) == 4) {
+            f[c] = __uint_as_float(h[c]);
+        } else {
+            const float2 p = pair_f32<InT>(h[c]);
+            f[2 * c] = p.x;
+            f[2 * c + 1] = p.y;
+        }
+    }
 }
 
 __global__ void build_inverse_map_kernel(const int32_t* __restrict__ sorted_ids,
@@ -40,8 +57,9 @@ __device__ __forceinline__ int64_t grid_token() {
 }
 
 // One CTA per (token, 512-channel chunk); each thread reduces 2 adjacent channels. Generic
-// path for N % 8 != 0 or unaligned rows. `pairs`: every row starts on a 4-byte boundary (N even, and
-// out2 itself: a view may start at any element), so that two channels are one load.
+// path for rows that 16 bytes do not divide or that are unaligned. `pairs`: 16-bit rows that all start
+// on a 4-byte boundary (N even, and out2 itself: a view may start at any element), so that two channels
+// are one load.
 template <typename InT, typename OutT>
 __global__ void __launch_bounds__(256)
 gather_reduce_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
@@ -57,20 +75,22 @@ gather_reduce_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ s
         if (r < 0) continue;
         const float w = topk_w[t * top_k + j];
         const InT* rowp = out2 + (int64_t)r * N + n;
-        if (pairs) {  // N is even: n + 1 < N
-            const float2 v = pair_f32<InT>(*reinterpret_cast<const uint32_t*>(rowp));
-            a0 = __fadd_rn(a0, __fmul_rn(w, v.x));
-            a1 = __fadd_rn(a1, __fmul_rn(w, v.y));
-        } else {
-            a0 = __fadd_rn(a0, __fmul_rn(w, row_f32(rowp[0])));
-            if (pair) a1 = __fadd_rn(a1, __fmul_rn(w, row_f32(rowp[1])));
+        if constexpr (sizeof(InT) == 2) {
+            if (pairs) {  // N is even: n + 1 < N
+                const float2 v = pair_f32<InT>(*reinterpret_cast<const uint32_t*>(rowp));
+                a0 = __fadd_rn(a0, __fmul_rn(w, v.x));
+                a1 = __fadd_rn(a1, __fmul_rn(w, v.y));
+                continue;
+            }
         }
+        a0 = __fadd_rn(a0, __fmul_rn(w, row_f32(rowp[0])));
+        if (pair) a1 = __fadd_rn(a1, __fmul_rn(w, row_f32(rowp[1])));
     }
     out[t * N + n] = (OutT)a0;
     if (pair) out[t * N + n + 1] = (OutT)a1;
 }
 
-// Vector path (N % 8 == 0, 16-byte aligned rows): one warp-row of 8-channel chunks per thread;
+// Vector path (16-byte aligned rows): 16 bytes of channels per thread (8, or 4 of fp32);
 // the top_k row indices and weights of the token are staged once per CTA, then every slot's
 // 16-byte row chunk is requested before the in-order accumulation.
 constexpr int kMaxTopK = 16;
@@ -79,6 +99,7 @@ __global__ void __launch_bounds__(256)
 gather_reduce_vec_kernel(const InT* __restrict__ out2, const int32_t* __restrict__ slot_to_row,
                          const float* __restrict__ topk_w, OutT* __restrict__ out, int64_t M,
                          int64_t N, int top_k) {
+    constexpr int kPer = 16 / sizeof(InT);
     __shared__ int32_t rows[kMaxTopK];
     __shared__ float wts[kMaxTopK];
     const int64_t t = grid_token();
@@ -88,34 +109,33 @@ gather_reduce_vec_kernel(const InT* __restrict__ out2, const int32_t* __restrict
         wts[threadIdx.x] = topk_w[t * top_k + threadIdx.x];
     }
     __syncthreads();
-    const int64_t n = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+    const int64_t n = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * kPer;
     if (n >= N) return;
     uint4 v[kMaxTopK];
 #pragma unroll
     for (int j = 0; j < kMaxTopK; ++j)
         if (j < top_k && rows[j] >= 0)
             v[j] = __ldg(reinterpret_cast<const uint4*>(out2 + (int64_t)rows[j] * N + n));
-    float acc[8];
+    float acc[kPer];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) acc[c] = 0.f;
+    for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
 #pragma unroll
     for (int j = 0; j < kMaxTopK; ++j) {
         if (j < top_k && rows[j] >= 0) {
             const float w = wts[j];
-            const uint32_t h[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+            float f[kPer];
+            unpack16<InT>(v[j], f);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float2 f = pair_f32<InT>(h[c]);
-                acc[2 * c] = __fadd_rn(acc[2 * c], __fmul_rn(w, f.x));
-                acc[2 * c + 1] = __fadd_rn(acc[2 * c + 1], __fmul_rn(w, f.y));
-            }
+            for (int c = 0; c < kPer; ++c) acc[c] = __fadd_rn(acc[c], __fmul_rn(w, f[c]));
         }
     }
     if constexpr (sizeof(OutT) == 4) {
         float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + t * N + n);
-        o[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        o[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+#pragma unroll
+        for (int c = 0; c < kPer; c += 4)
+            o[c / 4] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
     } else {
+        static_assert(sizeof(OutT) == 4 || kPer == 8, "16-bit results are made of 16-bit rows");
         uint4 o;
         uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
@@ -133,17 +153,18 @@ template <typename InT, typename OutT>
 static int launch_reduce(const InT* out2, const int32_t* slot_to_row, const float* topk_w,
                          OutT* out, int64_t M, int64_t N, int top_k, cudaStream_t stream) {
     if (M <= 0) return W4A8_OK;
-    const bool vec = N % 8 == 0 && top_k <= kMaxTopK &&
+    constexpr int kPer = 16 / sizeof(InT);
+    const bool vec = N % kPer == 0 && top_k <= kMaxTopK &&
                      (reinterpret_cast<uintptr_t>(out2) & 15) == 0 &&
                      (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     const int64_t z = (M + 65534) / 65535;
     const unsigned y = (unsigned)((M + z - 1) / z);
     if (vec) {
-        const dim3 grid((unsigned)((N / 8 + 255) / 256), y, (unsigned)z);
+        const dim3 grid((unsigned)((N / kPer + 255) / 256), y, (unsigned)z);
         gather_reduce_vec_kernel<InT, OutT><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w,
                                                                       out, M, N, top_k);
     } else {
-        const bool pairs = N % 2 == 0 && (reinterpret_cast<uintptr_t>(out2) & 3) == 0;
+        const bool pairs = sizeof(InT) == 2 && N % 2 == 0 && (reinterpret_cast<uintptr_t>(out2) & 3) == 0;
         const dim3 grid((unsigned)((N + 511) / 512), y, (unsigned)z);
         gather_reduce_kernel<InT, OutT><<<grid, 256, 0, stream>>>(out2, slot_to_row, topk_w, out,
                                                                   M, N, top_k, pairs);
@@ -216,6 +237,17 @@ extern "C" int w4a8_moe_gather_reduce_bf16(const void* out2, const int32_t* sort
     return w4a8::gather_reduce_entry<__nv_bfloat16>(out2, sorted_token_ids, topk_weights,
                                                     num_tokens_post_padded, out, M, N, P, top_k,
                                                     workspace, workspace_bytes, stream);
+}
+
+extern "C" int w4a8_moe_gather_reduce_f32(const void* out2, const int32_t* sorted_token_ids,
+                                          const float* topk_weights,
+                                          const int32_t* num_tokens_post_padded, float* out,
+                                          int64_t M, int64_t N, int64_t P, int64_t top_k,
+                                          void* workspace, size_t workspace_bytes,
+                                          w4a8_stream_t stream) {
+    return w4a8::gather_reduce_entry<float>(out2, sorted_token_ids, topk_weights,
+                                            num_tokens_post_padded, out, M, N, P, top_k, workspace,
+                                            workspace_bytes, stream);
 }
 
 namespace w4a8 {

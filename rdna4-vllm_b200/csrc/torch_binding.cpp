@@ -225,9 +225,10 @@ at::Tensor mmq_fp8_moe_gather_reduce_forward(const at::Tensor& out2,
                                              const at::Tensor& sorted_token_ids,
                                              const at::Tensor& topk_weights,
                                              const at::Tensor& ntp, int64_t top_k) {
-    const bool bf16 = out2.scalar_type() == at::kBFloat16;
-    TORCH_CHECK(out2.is_cuda() && (bf16 || out2.scalar_type() == at::kHalf) && out2.dim() == 2,
-                "out2 must be (P,N) fp16 or bf16 CUDA");
+    const at::ScalarType type = out2.scalar_type();
+    TORCH_CHECK(out2.is_cuda() && out2.dim() == 2 &&
+                    (type == at::kHalf || type == at::kBFloat16 || type == at::kFloat),
+                "out2 must be (P,N) fp16, bf16 or fp32 CUDA");
     TORCH_CHECK(sorted_token_ids.scalar_type() == at::kInt && ntp.scalar_type() == at::kInt &&
                     sorted_token_ids.dim() == 1 && ntp.numel() >= 1,
                 "sorted_token_ids (P,) / num_tokens_post_padded (1,) must be int32");
@@ -247,7 +248,9 @@ at::Tensor mmq_fp8_moe_gather_reduce_forward(const at::Tensor& out2,
     const c10::cuda::CUDAGuard guard(out2.device());
     auto out = at::empty({M, N}, out2.options().dtype(at::kFloat));
     auto ws = workspace(out2, w4a8_moe_gather_reduce_workspace_size(M, top_k));
-    const auto reduce = bf16 ? w4a8_moe_gather_reduce_bf16 : w4a8_moe_gather_reduce;
+    const auto reduce = type == at::kBFloat16 ? w4a8_moe_gather_reduce_bf16
+                        : type == at::kFloat  ? w4a8_moe_gather_reduce_f32
+                                              : w4a8_moe_gather_reduce;
     check_status(reduce(out2.data_ptr(), sorted_token_ids.data_ptr<int32_t>(),
                         topk_weights.data_ptr<float>(), ntp.data_ptr<int32_t>(),
                         out.data_ptr<float>(), M, N, sorted_token_ids.size(0), top_k,

@@ -129,7 +129,8 @@ def mmq_fp8_moe_gemm_scatter(x, w_packed, scales, sorted_token_ids, expert_ids,
 
 def mmq_fp8_moe_gather_reduce(out2, sorted_token_ids, topk_weights, num_tokens_post_padded,
                               top_k):
-    """Topk-weighted gather-reduce: (P, N) fp16 or bf16 rows -> (M, N) fp32, M = numel(w) // top_k."""
+    """Topk-weighted gather-reduce: (P, N) fp16, bf16 or fp32 rows -> (M, N) fp32,
+    M = numel(w) // top_k."""
     return torch.ops.w4a8_fp8_wmma.mmq_fp8_moe_gather_reduce(
         out2, sorted_token_ids, topk_weights, num_tokens_post_padded, top_k)
 

@@ -33,8 +33,8 @@ def run_fp8_block_moe(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w1_s:
     w2 (E, K, inter) e4m3, w1_s / w2_s (E, ceil(N/128), ceil(K/128)) fp32, inter a multiple of
     128. ``expert_map`` maps global expert ids to local ones (-1 = remote); remote slots
     contribute nothing. The steps are run_grouped_moe's: align, gate_up with SiLU (here also the
-    quantisation that down reads), down, gather-reduce; down's rows are bf16 when out_dtype is,
-    else fp16. Longer batches run in the same 4096-token chunks.
+    quantisation that down reads), down, gather-reduce; down's rows are fp16 or bf16 when
+    out_dtype is, else fp32. Longer batches run in the same 4096-token chunks.
     """
     if (x_scales is not None) and out_dtype is None:
         raise ValueError("run_fp8_block_moe: quantised x needs out_dtype")
@@ -61,7 +61,7 @@ def run_fp8_block_moe(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w1_s:
                                                        E_local)
     h, h_scales = fp8_block_moe_gemm1_silu(x, x_scales, w1, w1_s, sorted_ids, expert_ids, ntp,
                                            top_k, block_m)
-    rows = fp8_block_moe_gemm(h, h_scales, w2, w2_s, None, expert_ids, ntp, 1, block_m,
-                              torch.bfloat16 if out_dtype == torch.bfloat16 else torch.float16)
+    row_dtype = out_dtype if out_dtype in (torch.float16, torch.bfloat16) else torch.float32
+    rows = fp8_block_moe_gemm(h, h_scales, w2, w2_s, None, expert_ids, ntp, 1, block_m, row_dtype)
     tw = topk_weights.reshape(-1).to(torch.float32).contiguous()
     return mmq_fp8_moe_gather_reduce(rows, sorted_ids, tw, ntp, top_k).to(out_dtype)

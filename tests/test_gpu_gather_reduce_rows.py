@@ -83,3 +83,29 @@ def test_layer_refuses_weights_of_another_device(w4):
     for change in (dict(topk_weights=tw.cpu()), dict(topk_ids=ids.cpu())):
         with pytest.raises((RuntimeError, NotImplementedError)):
             run_fp8_block_moe(x, w1, w2, s1, s2, **{"topk_weights": tw, "topk_ids": ids, **change})
+
+
+@pytest.mark.parametrize("M,N,top_k", [(1, 4, 1), (7, 12, 2), (33, 1000, 8), (5, 1001, 3), (9, 6, 2), (4, 64, 17),
+                                       (700, 2048, 4), (70000, 4, 1), (70000, 3, 1)])
+@pytest.mark.parametrize("off", [0, 1, 4])
+def test_fp32_rows(w4, M, N, top_k, off):
+    """Through the vectorised kernel (N a multiple of 4, rows on 16 bytes) and the generic one; values
+    that fp16 does not hold."""
+    rows, s, n, tw = _case(M, N, top_k, FP32, M + N)
+    rows = rows * 1e6
+    base = torch.empty(rows.numel() + off, device="cuda")
+    view = base[off:].view_as(rows)
+    view.copy_(rows)
+    got = w4.mmq_fp8_moe_gather_reduce(view, s, tw, n, top_k)
+    assert got.dtype == FP32 and torch.equal(got, _expected(rows, s, tw, top_k))
+
+
+def test_fp32_rows_absent_slots(w4):
+    """Slots that no row holds (remote experts) add nothing; a token without any is zero."""
+    rows, s, _, tw = _case(6, 16, 2, FP32, 3)
+    n = torch.tensor([7], dtype=torch.int32, device="cuda")
+    here = torch.zeros(12, dtype=torch.bool, device="cuda")
+    here[s[:7].long()] = True
+    got = w4.mmq_fp8_moe_gather_reduce(rows, s, tw, n, 2)
+    kept = torch.where(here, tw, 0.0)
+    assert torch.equal(got, _expected(rows, s, kept, 2))
