@@ -127,9 +127,8 @@ __device__ __forceinline__ float scale_of(float amax) {
     return isinf(a) ? a : quotient(a, kE4m3Max, 1.f / kE4m3Max);
 }
 
-// kSign: zeros keep their sign (the residual of a -0 is +0). The steps of `quotient`, two values an
-// instruction.
-template <bool kSign>
+// The steps of `quotient`, two values an instruction. Zeros keep their sign (the residual of a -0 is
+// +0, and so would be its quotient).
 __device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale) {
     const float r = __frcp_rn(scale), s = isinf(scale) ? 0.f : -scale;
     const float2 r2 = make_float2(r, r), s2 = make_float2(s, s), none = make_float2(-0.f, -0.f);
@@ -139,7 +138,7 @@ __device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale) {
         const float2 v2 = make_float2(v[i], v[i + 1]);
         float2 y = ffma2(v2, r2, none);
         y = ffma2(ffma2(y, s2, v2), r2, y);
-        if (kSign) y = make_float2(copysignf(y.x, v2.x), copysignf(y.y, v2.y));
+        y = make_float2(copysignf(y.x, v2.x), copysignf(y.y, v2.y));
         u[i / 2] = f32x2_to_e4m3x2(y.x, y.y);
     }
     return make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
@@ -151,7 +150,7 @@ __device__ __forceinline__ uint2 quant_block_half(const float (&v)[8], float& s)
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
     s = scale_of(lanes_max<16>(amax));
-    return quant8<false>(v, s);
+    return quant8(v, s);
 }
 
 // K % 8 == 0 and aligned rows: 8 lanes per block, two vectors of 8 each. Bound by HBM: 8192 x 4096
@@ -192,7 +191,7 @@ act_quant_block_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
     if (sub == 0 && b < blocks) scales[b] = s;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-        if (ok[h]) *reinterpret_cast<uint2*>(q + at + h * 64) = quant8<true>(v[h], s);
+        if (ok[h]) *reinterpret_cast<uint2*>(q + at + h * 64) = quant8(v[h], s);
 }
 
 // The norm with the row in registers: kThreads threads per row, V vectors of 8 each (vector j of
