@@ -87,3 +87,20 @@ def test_fp32_rows_keep_their_bits(w4):
     h, hs = w4.fp8_block_moe_gemm1_silu(*w4.act_quant_fp8_block(x), w1, s1, s, e, n, 1, bm)
     rows = w4.fp8_block_moe_gemm(h, hs, w2, s2, None, e, n, 1, bm, out_dtype=FP32)
     assert torch.equal(y, rows[:T])
+
+
+def test_layer_of_one_chunk_past_65535_tokens(w4, monkeypatch):
+    """With chunking switched off; the first and the last tokens against the definition."""
+    from w4a8_fp8_wmma import fp8_block
+    monkeypatch.setattr(fp8_block, "APPLY_CHUNK", 0)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    T, E, k, H, I = 70000, 4, 2, 128, 128
+    x = _randn(g, T, H)
+    w1, w2, s1, s2 = _layer(g, E, H, I, 1.0)
+    ids, tw, _ = w4.route_topk(_randn(g, T, E), k)
+    y = fp8_block.run_fp8_block_moe(x, w1, w2, s1, s2, tw, ids)
+    assert bool(y.isfinite().all())
+    some = torch.cat([torch.arange(60), torch.arange(T - 60, T)]).cuda()
+    q, s = w4.act_quant_fp8_block(x[some])
+    want, tol = _definition(q, s, w1, w2, s1, s2, ids[some], tw[some], k)
+    assert bool(((y[some].double() - want).abs() <= tol).all())
