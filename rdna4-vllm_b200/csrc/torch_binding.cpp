@@ -230,7 +230,7 @@ at::Tensor mmq_fp8_moe_gather_reduce_forward(const at::Tensor& out2,
                     (type == at::kHalf || type == at::kBFloat16 || type == at::kFloat),
                 "out2 must be (P,N) fp16, bf16 or fp32 CUDA");
     TORCH_CHECK(sorted_token_ids.scalar_type() == at::kInt && ntp.scalar_type() == at::kInt &&
-                    sorted_token_ids.dim() == 1 && ntp.numel() >= 1,
+                    sorted_token_ids.numel() == sorted_token_ids.size(0) && ntp.numel() >= 1,
                 "sorted_token_ids (P,) / num_tokens_post_padded (1,) must be int32");
     TORCH_CHECK(topk_weights.scalar_type() == at::kFloat, "topk_weights must be fp32");
     TORCH_CHECK(sorted_token_ids.device() == out2.device() && ntp.device() == out2.device() &&

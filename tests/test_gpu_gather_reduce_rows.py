@@ -67,7 +67,8 @@ def test_refusals(w4):
     for args in bad:
         with pytest.raises((RuntimeError, NotImplementedError)):
             w4.mmq_fp8_moe_gather_reduce(*args, 2)
-    assert torch.equal(w4.mmq_fp8_moe_gather_reduce(rows, s, tw, n, 2), _expected(rows, s, tw, 2))
+    for ids in (s, s[:, None]):  # a column of ids is the ids
+        assert torch.equal(w4.mmq_fp8_moe_gather_reduce(rows, ids, tw, n, 2), _expected(rows, s, tw, 2))
 
 
 def test_layer_refuses_weights_of_another_device(w4):
