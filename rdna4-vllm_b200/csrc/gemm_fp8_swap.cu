@@ -23,10 +23,11 @@
 //
 // Measured: gate_up of 32 tokens over 256 experts (2048 -> 2 x 512, 346 MB) 61 us, 88 % of the
 // measured copy bandwidth; down of the same (174 MB) 32.9 us, 82 %: 8.8 tiles a CTA run as 9, and
-// padding rows are written too. Dense batches of up to 128 rows take 4 to 8 us on the device, most of
-// it latency: set-up 0.7, first data 0.9, the cluster's join 0.4. The set-up overlaps the end of the
-// work ahead in the stream (kEarly); without that, 1 x 4096 x 2048 took 8.0 us a call instead of 6.7,
-// 128 x 2048 x 4096 10.2 instead of 7.6, down 34.6.
+// padding rows are written too. Dense products of few tiles, replayed from a graph with weights that L2
+// does not hold, take 5.7 us (1 x 4096 x 2048), 7.1 (333 x 1001 x 1424) and 8.3 (128 x 2048 x 4096), most
+// of it latency: set-up 0.7, first data 0.9, the cluster's join 0.4. The set-up overlaps the end of the
+// work ahead in the stream (kEarly); without that they take 6.6, 8.1 and 9.4, and down 33.7 for 32.8.
+// Called one by one from Python the same three take 8.9 us each, the host's time for a call.
 //
 // Waits are bounded as in gemm_fp8_tc.cu: one that gives up leaves NaN in the tile's outputs.
 #include "fp8_tc.cuh"

@@ -26,7 +26,7 @@
 //
 // What bounds it: the 1000 W power cap, which takes the clock to 1.6 GHz and below in long runs.
 // 8192 x 8192 x 2048 takes 160 us, 1.72 PFLOP/s; gate_up of 4096 tokens over 256 experts (2048 -> 2 x
-// 512) 151 us, down of the same 94.5. In cycles a block of a 128 x 256 tile takes 930: MMA 590, to
+// 512) 151 us, down of the same 95. In cycles a block of a 128 x 256 tile takes 930: MMA 590, to
 // the fold and back 570, fold 400, over two accumulators, while its 48 KB come from L2 in 770 to 840.
 // Waits that poll rather than suspend make the way shorter and the runs 3 % longer. A pair of CTAs on
 // a tile of 256 x 256 (cta_group::2, 32 KB a block) was slower, 197 us against 173 for the first at

@@ -197,7 +197,7 @@ act_quant_block_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
 // The norm with the row in registers: kThreads threads per row, V vectors of 8 each (vector j of
 // thread t is j * kThreads + t, so 16 neighbours hold one block). A CTA walks rows with the
 // weights kept; rows of H % 8 == 0 elements, H <= 8 V kThreads, aligned. One pass over the rows,
-// bound by HBM: 16381 x 2048 bf16 with a residual in 42.0 us, 87 % of the measured copy bandwidth.
+// bound by HBM: 16381 x 2048 bf16 with a residual in 43.0 us, 85 % of the measured copy bandwidth.
 // CTAs for half or five eighths of the threads that an SM holds take 0.3 and 0.7 us more.
 template <typename T, typename W, int kThreads, int V>
 __global__ void __launch_bounds__(kThreads)
