@@ -30,8 +30,8 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float
 
 // One CTA: 16 rows x 128 outputs, thread = (row tid / 16, outputs tid % 16 + 16 j). fp32 FMAs on
 // the CUDA cores from staged fp32 copies; it takes every K and every alignment. Bound by the reads
-// of the staged copies, 16 a weight value: 1024 x 1024 x 1000 takes 224 us, where the tensor-core
-// kernels take 6.4 for K = 1024.
+// of the staged copies, 16 a weight value: 1024 x 1024 x 1000 takes 226 us, where the tensor-core
+// kernels take 6.2 on the device (8.9 a call) for K = 1024.
 template <bool SILU>
 __global__ void __launch_bounds__(256) fp8_simple_kernel(const Fp8Args a) {
     constexpr int kNw = SILU ? 256 : 128;  // weight rows of the tile
